@@ -21,6 +21,8 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "esmm.h")
 
 OK, ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_CUDA, ERR_TIMEOUT, ERR_IO, ERR_UNSUPPORTED, ERR_VERIFY, \
     ERR_TOO_LARGE, ERR_MISMATCH, ERR_BOUNDS = range(12)
+F32, F16, BF16, E4M3 = range(4)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 
 
 class EsmmError(RuntimeError):
@@ -75,6 +77,14 @@ _SIGNATURES = {
     "esmm_tf32x3_b_live_k": (_i, [_vp]),
     "esmm_tf32x3_workspace_bytes": (C.c_size_t, [_i, _i]),
     "esmm_sgemm_joint_tf32x3": (_i, [_i, _vp, _vp, _vp, _vp, _vp]),
+    "esmm_rmsnorm": (_i, [_i, _i, _i, _vp, _vp, _vp, _f, _vp, _i, _vp, _vp, _vp, _vp]),
+    "esmm_rmsnorm_backward_workspace_bytes": (C.c_size_t, [_i, _i]),
+    "esmm_rmsnorm_backward": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "esmm_quantize_rows": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp]),
+    "esmm_quantize_b": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp]),
+    "esmm_linear": (_i, [_i, _i, _i, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "esmm_epilogue_backward_workspace_bytes": (C.c_size_t, [_i, _i]),
+    "esmm_epilogue_backward": (_i, [_i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
     "esmm_cusparse_spmm": (_i, [_i, _i, _i, _vp, _vp, _vp, _i, C.POINTER(_f), C.POINTER(_f),
                                 C.POINTER(C.c_longlong)]),
     "esmm_plan_create": (_i, [_i, _i, _i, _vp, _i, C.POINTER(_vp)]),
@@ -223,6 +233,50 @@ def sgemm_joint_tf32x3(M: int, d_A: int, b: Tf32x3B, d_C: int, d_workspace: int,
     """Optional tensor-core variant (3xTF32; within a few 1e-6 of the FP32 path, not bit-identical): split of
     A + A patterns + product.  d_workspace holds tf32x3_workspace_bytes(M, b.K)."""
     check(lib().esmm_sgemm_joint_tf32x3(M, d_A, b.handle, d_C, d_workspace, stream), "esmm_sgemm_joint_tf32x3")
+
+
+def rmsnorm(M, K, dtype, d_x, d_residual, d_weight, eps, d_sum, out_dtype, d_out, d_scale: int = 0, d_rstd: int = 0,
+            stream: int = 0) -> None:
+    """h = x + residual (0: none) to d_sum (0: not kept); its root-mean-square norm times weight to d_out, in dtype or in E4M3 with
+    a scale per row."""
+    check(lib().esmm_rmsnorm(M, K, dtype, d_x, d_residual, d_weight, eps, d_sum, out_dtype, d_out, d_scale, d_rstd, stream),
+          "esmm_rmsnorm")
+
+
+def rmsnorm_backward_workspace_bytes(M: int, K: int) -> int:
+    return int(lib().esmm_rmsnorm_backward_workspace_bytes(M, K))
+
+
+def rmsnorm_backward(M, K, dtype, d_dout, d_h, d_weight, d_rstd, d_dsum, d_dx, d_dweight: int = 0, d_workspace: int = 0,
+                     stream: int = 0) -> None:
+    check(lib().esmm_rmsnorm_backward(M, K, dtype, d_dout, d_h, d_weight, d_rstd, d_dsum, d_dx, d_dweight, d_workspace, stream),
+          "esmm_rmsnorm_backward")
+
+
+def quantize_rows(M, K, dtype, d_x, d_out, d_scale, stream: int = 0) -> None:
+    check(lib().esmm_quantize_rows(M, K, dtype, d_x, d_out, d_scale, stream), "esmm_quantize_rows")
+
+
+def quantize_b(K, N, dtype, d_B, d_bt, d_scale, stream: int = 0) -> None:
+    """B (K x N) as N x K e4m3 with a scale per column of B: the B of an 8-bit linear(trans_b=1)."""
+    check(lib().esmm_quantize_b(K, N, dtype, d_B, d_bt, d_scale, stream), "esmm_quantize_b")
+
+
+def linear(M, N, K, dtype, d_A, d_B, out_dtype, d_C, trans_a: int = 0, trans_b: int = 0, a_scale: int = 0, b_scale: int = 0,
+           bias: int = 0, residual: int = 0, pre: int = 0, activation: int = ACT_NONE, stream: int = 0) -> None:
+    """C = act(a_scale b_scale (op(A) op(B)) + bias) + residual on the tensor cores; `pre` keeps the values before the activation."""
+    check(lib().esmm_linear(M, N, K, dtype, d_A, trans_a, d_B, trans_b, out_dtype, d_C, a_scale, b_scale, bias, residual, pre,
+                            activation, stream), "esmm_linear")
+
+
+def epilogue_backward_workspace_bytes(M: int, N: int) -> int:
+    return int(lib().esmm_epilogue_backward_workspace_bytes(M, N))
+
+
+def epilogue_backward(M, N, dtype, d_dC, d_pre, activation, d_dZ, d_dbias: int = 0, d_workspace: int = 0, stream: int = 0) -> None:
+    """dZ = dC act'(pre) and dbias, the sums of its columns."""
+    check(lib().esmm_epilogue_backward(M, N, dtype, d_dC, d_pre, activation, d_dZ, d_dbias, d_workspace, stream),
+          "esmm_epilogue_backward")
 
 
 def device_status(stream: int = 0) -> None:

@@ -1,0 +1,798 @@
+// Dense matrix product with its epilogue on the 5th-generation tensor cores (tcgen05, sm_100a), for 16-bit and 8-bit operands:
+//
+//   C = act(a_scale_i b_scale_j sum_k op(A)_ik op(B)_kj + bias_j) + residual_ij,   FP32 accumulation in tensor memory, one rounding.
+//
+// Operands are read as they lie.  A K step is 128 bytes of K (64 16-bit or 128 e4m3 values).  An operand whose K runs along
+// memory (A of M x K, B stored transposed as N x K) comes as boxes of 128 bytes x rows with the 128-byte swizzle, the canonical K-major
+// layout; one whose other index does (A stored as K x M, B of K x N, 16-bit only) as boxes of 64 values x 64 k, the canonical
+// MN-major layout: eight k of 64 values are 1024 bytes, the next 64 values follow a box later.  So neither the forward product nor
+// its gradients (dA = dZ B^T, dB = A^T dZ) need a transposed copy of anything.
+//
+// Two kernels:
+//   esmm_linear_pair_kernel<NB, F8>   large products.  Persistent, a cluster of two CTAs per 256 x NB tile (cta_group::2 MMAs): each CTA
+//       fetches its 128 rows of A and NB / 2 columns of B into a ring, one thread of the even CTA issues the MMAs, eight
+//       epilogue warps per CTA drain one of two accumulators in tensor memory while the other is filled.
+//   esmm_linear_split_kernel<NB, F8>  few rows or few tiles: one CTA per 128 x NB tile and part of K, the parts of a tile being one
+//       cluster.  The CTAs add up their accumulators through distributed shared memory in a fixed order, each of them finishing a
+//       share of the tile's outputs: no workspace, no atomics, the same bits on every call.  Its cost is the operands' bytes: all
+//       SMs stream the weights whatever the number of tokens, and rows of A that do not exist are not fetched.
+// Every wait is bounded, as in the other kernels; tensor memory is freed on every path out.
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "esmm_dtypes.cuh"
+#include "esmm_gemm_shared.cuh"
+
+namespace esmm {
+
+struct LinearParams {
+    int M, N, ksteps;                    // K in steps of 128 bytes
+    int tiles_m, tiles_n, num_tiles;
+    int group_m;
+    int a_boxes, b_boxes;                // copies per stage and operand
+    int a_k_major, b_k_major;
+    int k_elems;                         // elements of K per step
+    int stages;
+    int a_stage_bytes;                   // split kernel: of A's part of a stage
+    uint32_t idesc;
+    uint32_t a_lbo, b_lbo;               // leading byte offset of the descriptors, in place
+    uint32_t a_step, b_step;             // from one MMA to the next along K, in 16-byte units
+    int bf16;                            // type of C, bias, residual and pre: bfloat16 or float16
+    int activation, has_pre, has_residual;
+    const float *a_scale, *b_scale;
+    const void *bias;
+    const void *residual;                // split kernel
+    void *pre, *C;                       // split kernel
+    int *status;
+};
+
+struct LinearMaps {
+    CUtensorMap a, b;
+    CUtensorMap c, residual, pre;        // pair kernel: boxes of 64 columns x 32 rows, 128-byte swizzle
+};
+
+constexpr int L_KBYTES = 128;            // bytes of K per step
+constexpr uint32_t L_DESC_HI = 64u | (1u << 14) | (2u << 29);   // eight rows (or k) of 128 bytes every 1024 bytes, version 1, 128-byte swizzle
+
+template <bool PAIR, bool F8>
+__device__ __forceinline__ void linear_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate)
+{
+#define ESMM_LINEAR_MMA(GROUP, KIND, ZEROS)                                                                            \
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                         \
+                 "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"                         \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %3, " ZEROS ", p;\n\t}\n" ::"r"(tmem_d), \
+                 "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(L_DESC_HI), "r"(0u)                            \
+                 : "memory")
+    if constexpr (PAIR && F8) ESMM_LINEAR_MMA("2", "f8f6f4", "{%6, %6, %6, %6, %6, %6, %6, %6}");
+    else if constexpr (PAIR) ESMM_LINEAR_MMA("2", "f16", "{%6, %6, %6, %6, %6, %6, %6, %6}");
+    else if constexpr (F8) ESMM_LINEAR_MMA("1", "f8f6f4", "{%6, %6, %6, %6}");
+    else ESMM_LINEAR_MMA("1", "f16", "{%6, %6, %6, %6}");
+#undef ESMM_LINEAR_MMA
+}
+
+// arrives on the barrier (at this offset in both CTAs of a pair) once the MMAs issued so far are complete
+template <bool PAIR>
+__device__ __forceinline__ void linear_commit(uint32_t bar)
+{
+    if constexpr (PAIR) {
+        const uint16_t mask = 3;
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"(mask)
+                     : "memory");
+    } else {
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    }
+}
+
+__device__ __forceinline__ void linear_tmem_ld(uint32_t taddr, float (&v)[32])
+{
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void linear_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void linear_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t linear_cta_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void linear_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t linear_map_to_cta(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void linear_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar)
+{
+    if constexpr (PAIR)   // the bytes are counted on a barrier that may lie in the pair's other CTA
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else
+        tma_load_2d(dst, map, x, y, bar);
+}
+
+// After a wait that ran out: copies and MMAs of this CTA that are still in flight are over long before this is.
+__device__ __forceinline__ void linear_settle()
+{
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
+// The copies of one K step: lanes 0 .. a_boxes - 1 fetch A, lanes 2 .. 2 + b_boxes - 1 fetch B.  row_a, row_b: first row of op(A) and
+// column of op(B) of this CTA's part of the tile.
+template <bool PAIR>
+__device__ __forceinline__ void linear_load_step(const LinearParams &p, const LinearMaps &maps, int lane, int step, int row_a, int row_b,
+                                                 uint32_t dst_a, uint32_t dst_b, uint32_t bar)
+{
+    const bool is_b = lane >= 2;
+    const int i = lane & 1;
+    if (lane >= 4 || i >= (is_b ? p.b_boxes : p.a_boxes)) return;
+    const int k = step * p.k_elems, r = (is_b ? row_b : row_a) + 64 * i;
+    const bool k_major = is_b ? p.b_k_major : p.a_k_major;
+    linear_load<PAIR>((is_b ? dst_b : dst_a) + 8192u * (uint32_t)i, is_b ? &maps.b : &maps.a, k_major ? k : r, k_major ? r : k, bar);
+}
+
+// z: 32 sums of one row, columns c0 .. c0 + 31; scale and bias by column in shared memory.
+template <int ACT>
+__device__ __forceinline__ void linear_finish(float (&z)[32])
+{
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] = activate<ACT>(z[j]);
+}
+
+// ----------------------------------------------------------------------------------------------------------------------------
+// Pair kernel
+// ----------------------------------------------------------------------------------------------------------------------------
+constexpr int LP_EPI_WARPS = 8;
+constexpr int LP_THREADS = (4 + LP_EPI_WARPS) * 32;
+constexpr int LP_STAGING = 2 * 4096;              // per epilogue warp: two boxes of 32 rows x 64 16-bit columns
+constexpr int LP_MAX_STAGES = 8;
+template <int NB> struct LinearPairCfg {
+    static constexpr int A_BYTES = 128 * L_KBYTES, B_BYTES = (NB / 2) * L_KBYTES;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = NB == 256 ? 5 : 6;
+    static constexpr int RING = STAGES * STAGE_BYTES;
+    static constexpr int STAGING_OFF = RING;
+    static constexpr int COLUMN_OFF = STAGING_OFF + LP_EPI_WARPS * LP_STAGING;   // per epilogue warp: 32 scales, 32 biases
+    static constexpr int BAR_OFF = COLUMN_OFF + LP_EPI_WARPS * 256;
+    static constexpr int SMEM = BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
+    static constexpr int TMEM_COLS = 2 * NB;
+    static_assert(SMEM <= SMEM_LIMIT && STAGES <= LP_MAX_STAGES, "shared memory of a CTA");
+};
+
+template <int NB, bool F8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LP_THREADS, 1)
+esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p)
+{
+    using Cfg = LinearPairCfg<NB>;
+    extern __shared__ __align__(1024) char smem[];
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::BAR_OFF);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + LP_MAX_STAGES), accf0 = smem_u32(bars + 2 * LP_MAX_STAGES),
+                   acce0 = smem_u32(bars + 2 * LP_MAX_STAGES + 2), res0 = smem_u32(bars + 2 * LP_MAX_STAGES + 4);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(abort_flag + 1));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = linear_cta_rank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);                   // (even CTA) its producer; bytes of both CTAs' copies
+            mbar_init(empty0 + 8 * s, 1);                  // one commit per stage, delivered to both CTAs
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(accf0 + 8 * b, 1);
+            mbar_init(acce0 + 8 * b, 2 * LP_EPI_WARPS);    // (even CTA) the epilogue warps of both CTAs
+        }
+        for (int w = 0; w < LP_EPI_WARPS; ++w) mbar_init(res0 + 8 * w, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(Cfg::TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    linear_fence_before();
+    __syncthreads();
+    linear_cluster_sync();
+    linear_fence_after();
+    grid_dependency_wait();
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---------------- producer ----------------
+        if (lane == 0) tma_prefetch_descriptor(&maps.a);
+        if (lane == 2) tma_prefetch_descriptor(&maps.b);
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
+            int tm, tn;
+            tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
+            const int row_a = tm * 256 + (int)rank * 128, row_b = tn * NB + (int)rank * (NB / 2);
+            for (int step = 0; step < p.ksteps; ++step) {
+                ok = mbar_wait(empty0 + 8 * slot, phase ^ 1, abort_flag);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * Cfg::STAGE_BYTES);
+                __syncwarp();
+                const uint32_t dst = smem_u32(smem) + (uint32_t)slot * Cfg::STAGE_BYTES;
+                linear_load_step<true>(p, maps, lane, step, row_a, row_b, dst, dst + Cfg::A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
+                if (++slot == Cfg::STAGES) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issue: one thread of the even CTA, for both CTAs ----------------
+        if (leader && lane == 0) {
+            int slot = 0;
+            uint32_t phase = 0, turn = 0;
+            bool landed = false;
+            const uint32_t ring = (smem_u32(smem) & 0x3FFFFu) >> 4;
+            for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs, ++turn) {
+                const uint32_t ab = turn & 1u;
+                ok = mbar_wait(acce0 + 8 * ab, ((turn >> 1) & 1u) ^ 1u, abort_flag);   // drained in both CTAs
+                if (!ok) break;
+                linear_fence_after();
+                const uint32_t d = tmem + ab * (uint32_t)NB;
+                for (int step = 0; step < p.ksteps; ++step) {
+                    if (!landed) ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
+                    if (!ok) break;
+                    const uint32_t a = (ring + (uint32_t)slot * (Cfg::STAGE_BYTES >> 4)) | p.a_lbo;
+                    const uint32_t b = (ring + (uint32_t)slot * (Cfg::STAGE_BYTES >> 4) + (Cfg::A_BYTES >> 4)) | p.b_lbo;
+                    const int nslot = slot + 1 == Cfg::STAGES ? 0 : slot + 1;
+                    linear_mma<true, F8>(d, a, b, p.idesc, step ? 1u : 0u);
+                    // (a wait costs this thread time even where the data is there: ask while the pipe has work)
+                    landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
+#pragma unroll
+                    for (uint32_t j = 1; j < 4; ++j) linear_mma<true, F8>(d, a + j * p.a_step, b + j * p.b_step, p.idesc, 1u);
+                    linear_commit<true>(empty0 + 8 * slot);
+                    if (++slot == Cfg::STAGES) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                linear_commit<true>(accf0 + 8 * ab);
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: a row per thread, 64 columns at a time through the warp's staging boxes ----------------
+        const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns NB / 2 * half ..
+        constexpr int CHUNKS = NB / 128;
+        char *box = smem + Cfg::STAGING_OFF + w * LP_STAGING;
+        float *col_scale = reinterpret_cast<float *>(smem + Cfg::COLUMN_OFF + w * 256), *col_bias = col_scale + 32;
+        const uint32_t res_bar = res0 + 8 * w;
+        uint32_t turn = 0, res_phase = 0;
+        for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs, ++turn) {
+            int tm, tn;
+            tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
+            const int row0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tn * NB + half * (NB / 2);
+            const uint32_t ab = turn & 1u;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the boxes are free again
+            if (p.has_residual && row0 < p.M && col0 < p.N) {
+                if (lane == 0) {
+                    const int boxes = CHUNKS == 2 && col0 + 64 < p.N ? 2 : 1;
+                    mbar_arrive_expect_tx(res_bar, 4096u * (uint32_t)boxes);
+                    for (int c = 0; c < boxes; ++c) tma_load_2d(smem_u32(box) + 4096u * c, &maps.residual, col0 + 64 * c, row0, res_bar);
+                }
+            }
+            __syncwarp();
+            const float sa = p.a_scale && row0 + lane < p.M ? p.a_scale[row0 + lane] : 1.0f;
+            ok = mbar_wait(accf0 + 8 * ab, (turn >> 1) & 1u, abort_flag);
+            if (!ok) break;
+            linear_fence_after();
+            if (p.has_residual && row0 < p.M && col0 < p.N) {
+                ok = mbar_wait(res_bar, res_phase, abort_flag);
+                if (!ok) break;
+                res_phase ^= 1u;
+            }
+#pragma unroll 1
+            for (int c = 0; c < CHUNKS; ++c) {
+                const int col = col0 + 64 * c;
+                char *mine = box + 4096 * c + lane * 128;
+                uint32_t pre[32];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float z[32];
+                    const int cj = col + 32 * h + lane;
+                    float b = 0.0f;
+                    if (p.bias && cj < p.N)
+                        b = p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[cj]) : __half2float(static_cast<const __half *>(p.bias)[cj]);
+                    __syncwarp();
+                    col_scale[lane] = p.b_scale && cj < p.N ? p.b_scale[cj] : 1.0f;
+                    col_bias[lane] = b;
+                    __syncwarp();
+                    linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + ab * (uint32_t)NB + (uint32_t)(half * (NB / 2) + 64 * c + 32 * h), z);
+                    if (c == CHUNKS - 1 && h == 1) {              // the accumulator is read: the next but one tile may have it
+                        linear_fence_before();
+                        __syncwarp();
+                        if (lane == 0)
+                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(linear_map_to_cta(acce0 + 8 * ab, 0)) : "memory");
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(col_scale + j), b4 = *reinterpret_cast<const float4 *>(col_bias + j);
+                        z[j] = fmaf(z[j] * sa, s4.x, b4.x);
+                        z[j + 1] = fmaf(z[j + 1] * sa, s4.y, b4.y);
+                        z[j + 2] = fmaf(z[j + 2] * sa, s4.z, b4.z);
+                        z[j + 3] = fmaf(z[j + 3] * sa, s4.w, b4.w);
+                    }
+                    if (p.has_pre) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) pre[16 * h + j] = p.bf16 ? pack_bf16(z[2 * j], z[2 * j + 1]) : pack_f16(z[2 * j], z[2 * j + 1]);
+                    }
+                    with_activation(p.activation, [&](auto tag) { linear_finish<decltype(tag)::value>(z); });
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {                 // 16 bytes = 8 columns; chunk x of row r lies at x ^ (r & 7)
+                        uint4 *at = reinterpret_cast<uint4 *>(mine + (((4 * h + j) ^ (lane & 7)) << 4));
+                        if (p.has_residual) {
+                            const uint4 r = *at;
+                            const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = p.bf16 ? unpack_bf16(rw[e]) : unpack_f16(rw[e]);
+                                z[8 * j + 2 * e] += f.x;
+                                z[8 * j + 2 * e + 1] += f.y;
+                            }
+                        }
+                        uint32_t o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[e] = p.bf16 ? pack_bf16(z[8 * j + 2 * e], z[8 * j + 2 * e + 1]) : pack_f16(z[8 * j + 2 * e], z[8 * j + 2 * e + 1]);
+                        *at = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                const bool inside = row0 < p.M && col < p.N;      // (a box wholly outside C is not stored; the rest is clipped)
+                if (lane == 0) {
+                    if (inside)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&maps.c), "r"(col), "r"(row0),
+                                     "r"(smem_u32(box) + 4096u * c)
+                                     : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+                if (p.has_pre) {
+                    // the values before the activation take the same box once C's have left it
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<uint4 *>(mine + ((j ^ (lane & 7)) << 4)) = make_uint4(pre[4 * j], pre[4 * j + 1], pre[4 * j + 2], pre[4 * j + 3]);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (inside)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&maps.pre), "r"(col), "r"(row0),
+                                         "r"(smem_u32(box) + 4096u * c)
+                                         : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+
+    if (!ok) {
+        linear_settle();
+        if (lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
+    }
+    linear_fence_before();
+    __syncthreads();
+    linear_cluster_sync();        // nothing of the other CTA is touched after this
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS));
+}
+
+// ----------------------------------------------------------------------------------------------------------------------------
+// Split kernel
+// ----------------------------------------------------------------------------------------------------------------------------
+constexpr int LS_THREADS = 192;                   // warps 0-3 drain the accumulator, 4 copies, 5 issues the MMAs
+constexpr int LS_MAX_STAGES = 16;
+constexpr int LS_MAX_SPLIT = 8;
+
+// shared memory: ring of A, ring of B (the sums lie over both after the last MMA) | barriers, flags
+__host__ __device__ constexpr int ls_red_bytes(int rows, int nb) { return rows * (nb + 4) * 4; }
+
+template <int NB, bool F8>
+__global__ void __launch_bounds__(LS_THREADS)
+esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p, const int split, const int bar_off)
+{
+    extern __shared__ __align__(1024) char smem[];
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + bar_off);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + LS_MAX_STAGES), accf = smem_u32(bars + 2 * LS_MAX_STAGES);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 2 * LS_MAX_STAGES + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(const_cast<int *>(abort_flag + 1));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)linear_cta_rank();
+    const int tile = blockIdx.x / split;
+    int tm, tn;
+    tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
+    const int s0 = (int)((long)p.ksteps * rank / split), s1 = (int)((long)p.ksteps * (rank + 1) / split);   // this CTA's K steps, one at least
+    const int row0 = tm * 128, col0 = tn * NB, rows = min(128, p.M - row0);
+    constexpr int B_BYTES = NB * L_KBYTES;
+    const uint32_t a_ring = smem_u32(smem), b_ring = a_ring + (uint32_t)(p.stages * p.a_stage_bytes);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(accf, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(NB));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    linear_fence_before();
+    __syncthreads();
+    linear_fence_after();
+    grid_dependency_wait();
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 4) {
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int step = s0; step < s1; ++step) {
+            ok = mbar_wait(empty0 + 8 * slot, phase ^ 1, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, (uint32_t)(p.a_stage_bytes + B_BYTES));
+            __syncwarp();
+            linear_load_step<false>(p, maps, lane, step, row0, col0, a_ring + (uint32_t)(slot * p.a_stage_bytes), b_ring + (uint32_t)(slot * B_BYTES),
+                                    full0 + 8 * slot);
+            if (++slot == p.stages) {
+                slot = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            int slot = 0;
+            uint32_t phase = 0;
+            for (int step = s0; step < s1; ++step) {
+                ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
+                if (!ok) break;
+                const uint32_t a = (((a_ring + (uint32_t)(slot * p.a_stage_bytes)) & 0x3FFFFu) >> 4) | p.a_lbo;
+                const uint32_t b = (((b_ring + (uint32_t)(slot * B_BYTES)) & 0x3FFFFu) >> 4) | p.b_lbo;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    linear_mma<false, F8>(tmem, a + j * p.a_step, b + j * p.b_step, p.idesc, step > s0 || j ? 1u : 0u);
+                linear_commit<false>(empty0 + 8 * slot);
+                if (++slot == p.stages) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            if (ok) linear_commit<false>(accf);
+        }
+    } else if (warp < 4) {
+        // The sums of the rows that exist, to shared memory: 16 bytes apart beyond their length, so that the stores of eight threads
+        // (eight rows) fall on all banks.  The ring is free: every copy has landed and every MMA has read it.
+        ok = mbar_wait(accf, 0, abort_flag);
+        if (ok && warp * 32 < rows) {
+            linear_fence_after();
+            float *red = reinterpret_cast<float *>(smem) + (size_t)(warp * 32 + lane) * (NB + 4);
+            const bool mine = warp * 32 + lane < rows;
+#pragma unroll
+            for (int c = 0; c < NB; c += 32) {
+                float z[32];
+                linear_tmem_ld(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, z);
+                if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(red + c + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+                }
+            }
+            linear_fence_before();
+        }
+    }
+    if (!ok) {
+        linear_settle();
+        if (lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
+    }
+    __syncwarp();
+    linear_cluster_sync();       // all parts' sums are in their CTAs' shared memory
+
+    // Eight outputs of a row at a time: the parts' sums in the order of K, the epilogue, one 16-byte store.
+    const int groups = rows * (NB / 8);
+    const uint32_t red0 = smem_u32(smem);
+    for (int g = rank * LS_THREADS + threadIdx.x; g < groups; g += split * LS_THREADS) {
+        const int r = g / (NB / 8), c = (g - r * (NB / 8)) * 8, row = row0 + r, col = col0 + c;
+        if (col >= p.N) continue;
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = 0.0f;
+        const uint32_t at = red0 + (uint32_t)((r * (NB + 4) + c) * 4);
+        for (int part = 0; part < split; ++part) {
+            const uint32_t from = linear_map_to_cta(at, (uint32_t)part);
+            float4 u, v;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(from));
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from + 16));
+            z[0] += u.x, z[1] += u.y, z[2] += u.z, z[3] += u.w;
+            z[4] += v.x, z[5] += v.y, z[6] += v.z, z[7] += v.w;
+        }
+        const size_t off = (size_t)row * p.N + col;
+        auto unpack2 = [&](uint32_t v) { return p.bf16 ? unpack_bf16(v) : unpack_f16(v); };
+        auto pack2 = [&](float lo, float hi) { return p.bf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); };
+        if (p.a_scale) {
+            const float sa = p.a_scale[row];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] *= sa;
+        }
+        if (p.b_scale) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] *= p.b_scale[col + j];
+        }
+        if (p.bias) {
+            const uint4 b = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.bias) + (size_t)col * 2);
+            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2(bw[e]);
+                z[2 * e] += f.x;
+                z[2 * e + 1] += f.y;
+            }
+        }
+        const bool inside = bounds_ok(off + 8 <= (size_t)p.M * p.N, p.status, 64);   // checked build: site 64
+        if (p.has_pre && inside)
+            *reinterpret_cast<uint4 *>(static_cast<char *>(p.pre) + off * 2) = make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7]));
+        with_activation(p.activation, [&](auto tag) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
+        });
+        if (p.has_residual) {
+            const uint4 b = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.residual) + off * 2);
+            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2(bw[e]);
+                z[2 * e] += f.x;
+                z[2 * e + 1] += f.y;
+            }
+        }
+        if (inside)
+            *reinterpret_cast<uint4 *>(static_cast<char *>(p.C) + off * 2) = make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7]));
+    }
+    linear_cluster_sync();       // (the others may still read this CTA's sums)
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB));
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------------------
+// Once per device: the SM count and the shared-memory allowance of every kernel.
+static int linear_prepare(int dev, int *sms)
+{
+    static std::mutex mu;
+    static int count[64];
+    if (dev < 0 || dev >= 64) return record_cuda_error_text("esmm_linear: device ordinal out of range");
+    std::lock_guard<std::mutex> lock(mu);
+    if (!count[dev]) {
+        int n = 0;
+        ESMM_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        auto allow = [](auto kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<256, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<256, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<128, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<128, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<128, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<128, true>, SMEM_LIMIT));
+        count[dev] = n;
+    }
+    *sms = count[dev];
+    return ESMM_OK;
+}
+
+// Row-major matrix of `outer` rows x `inner` elements of `dtype`, 128-byte swizzle.
+static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner, long outer, int box_inner, int box_outer)
+{
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return record_cuda_error_text("cuTensorMapEncodeTiled entry point not available");
+    const int size = dtype_bytes(dtype);
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+    cuuint64_t strides[1] = {(cuuint64_t)inner * size};
+    cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
+    cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType type = dtype == ESMM_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : dtype == ESMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char buf[96];
+        snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+        return record_cuda_error_text(buf);
+    }
+    return ESMM_OK;
+}
+
+struct LinearChoice {
+    int pair_nb;          // 256, 128: the pair kernel's tile; 0: the split kernel
+    int nb, split;        // split kernel
+};
+
+// Which kernel, by the time per SM that each would take, in K steps of a 128 x 128 tile (64 cycles of MMA per SM at 16 bits).
+static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
+{
+    LinearChoice c;
+    const int pairs = std::max(1, sms / 2);
+    auto rounds = [](long items, long slots) { return (double)((items + slots - 1) / slots); };
+    // the pair kernel: whole rounds of tiles, and the last tile's epilogue
+    const double t256 = rounds((long)ceil_div(M, 256) * ceil_div(N, 256), pairs) * 2.0 * ksteps + 8.0;
+    const double t128 = rounds((long)ceil_div(M, 256) * ceil_div(N, 128), pairs) * 1.2 * ksteps + 6.0;
+    // the split kernel: parts of K so that all SMs have work
+    c.nb = 128;
+    const long tiles = (long)ceil_div(M, 128) * ceil_div(N, c.nb);
+    c.split = (int)std::max(1L, std::min<long>(LS_MAX_SPLIT, 2L * sms / tiles));
+    c.split = std::min(c.split, std::max(1, ksteps / 4));
+    const double ts = rounds(tiles * c.split, 2L * sms) * 2.6 * (double)ceil_div(ksteps, c.split) + 10.0;
+    c.pair_nb = M <= 128 || ts <= std::min(t256, t128) ? 0 : t256 <= t128 ? 256 : 128;
+    const int forced = tuning_get("LINEAR_PAIR", -1);
+    if (forced == 0 || forced == 128 || forced == 256) c.pair_nb = forced;
+    const int forced_split = tuning_get("LINEAR_SPLIT", 0);
+    if (forced_split >= 1 && forced_split <= LS_MAX_SPLIT) c.split = std::min(forced_split, ksteps);
+    const int forced_nb = tuning_get("LINEAR_COLUMNS", 0);
+    if (forced_nb == 64 || forced_nb == 128) c.nb = forced_nb;
+    return c;
+}
+
+}  // namespace esmm
+
+extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int trans_a, const void *d_B, int trans_b, int out_dtype, void *d_C,
+                           const float *d_a_scale, const float *d_b_scale, const void *d_bias, const void *d_residual, void *d_pre, int activation,
+                           void *stream_)
+{
+    using namespace esmm;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    if (!d_A || !d_B || !d_C) return ESMM_ERR_NULL;
+    const bool f8 = dtype == ESMM_E4M3;
+    if (!f8 && dtype != ESMM_F16 && dtype != ESMM_BF16) return ESMM_ERR_UNSUPPORTED;
+    if (f8 ? (out_dtype != ESMM_F16 && out_dtype != ESMM_BF16) : out_dtype != dtype) return ESMM_ERR_UNSUPPORTED;
+    if (f8 && (trans_a || !trans_b)) return ESMM_ERR_UNSUPPORTED;
+    if (trans_a && trans_b) return ESMM_ERR_UNSUPPORTED;
+    if (!activation_known(activation)) return ESMM_ERR_UNSUPPORTED;
+    if (M <= 0 || N <= 0 || K <= 0 || N % 8) return ESMM_ERR_SHAPE;
+    // rows of 16 bytes: A's are K (or, transposed, M) long, B's N or K
+    const int per16 = f8 ? 16 : 8;
+    if ((trans_a ? M : K) % per16 || (trans_b ? K % per16 : 0)) return ESMM_ERR_SHAPE;
+    if (((uintptr_t)d_A | (uintptr_t)d_B | (uintptr_t)d_C | (uintptr_t)d_bias | (uintptr_t)d_residual | (uintptr_t)d_pre) & 15) return ESMM_ERR_ALIGN;
+    if (((uintptr_t)d_a_scale | (uintptr_t)d_b_scale) & 3) return ESMM_ERR_ALIGN;
+
+    int dev = 0, sms = 0;
+    ESMM_CUDA_TRY(cudaGetDevice(&dev));
+    int st = linear_prepare(dev, &sms);
+    if (st != ESMM_OK) return st;
+
+    LinearParams p;
+    memset(&p, 0, sizeof p);
+    p.M = M;
+    p.N = N;
+    p.k_elems = f8 ? 128 : 64;
+    p.ksteps = ceil_div(K, p.k_elems);
+    p.a_k_major = !trans_a;
+    p.b_k_major = trans_b != 0;
+    // K-major: the next MMA's 32 bytes of K lie in the same rows; MN-major: its 16 k are two groups of 1024 bytes on
+    p.a_step = p.a_k_major ? 2u : 128u;
+    p.b_step = p.b_k_major ? 2u : 128u;
+    p.a_lbo = (p.a_k_major ? 1u : 8192u >> 4) << 16;
+    p.b_lbo = (p.b_k_major ? 1u : 8192u >> 4) << 16;
+    p.bf16 = out_dtype == ESMM_BF16;
+    p.activation = activation;
+    p.has_pre = d_pre != nullptr;
+    p.has_residual = d_residual != nullptr;
+    p.a_scale = d_a_scale;
+    p.b_scale = d_b_scale;
+    p.bias = d_bias;
+    p.residual = d_residual;
+    p.pre = d_pre;
+    p.C = d_C;
+    p.group_m = GROUP_M;
+    p.status = device_status_ptr();
+    if (!p.status) return ESMM_ERR_CUDA;
+
+    const LinearChoice choice = linear_choose(M, N, p.ksteps, sms);
+    const int rows_a = 128;                                                 // rows of A per CTA
+    const int cols_b = choice.pair_nb ? choice.pair_nb / 2 : choice.nb;     // columns of B per CTA
+    // few rows: boxes of as many as there are (what the MMA reads past them is never looked at)
+    int a_box_rows = rows_a;
+    if (!choice.pair_nb && p.a_k_major && M < rows_a) a_box_rows = ceil_div(M, 8) * 8;
+    p.a_boxes = p.a_k_major ? 1 : rows_a / 64;
+    p.b_boxes = p.b_k_major ? 1 : cols_b / 64;
+    // D = F32; A and B: F16 0, BF16 1, E4M3 0; bits 15, 16: MN-major; N >> 3, M >> 4
+    const uint32_t ab_type = dtype == ESMM_BF16 ? 1u : 0u;
+    const uint32_t mma_m = choice.pair_nb ? 256u : 128u, mma_n = (uint32_t)(choice.pair_nb ? choice.pair_nb : choice.nb);
+    p.idesc = (1u << 4) | (ab_type << 7) | (ab_type << 10) | ((p.a_k_major ? 0u : 1u) << 15) | ((p.b_k_major ? 0u : 1u) << 16) |
+              ((mma_n >> 3) << 17) | ((mma_m >> 4) << 24);
+
+    LinearMaps maps;
+    memset(&maps, 0, sizeof maps);
+    st = p.a_k_major ? linear_map(&maps.a, dtype, d_A, K, M, p.k_elems, a_box_rows) : linear_map(&maps.a, dtype, d_A, M, K, 64, 64);
+    if (!st) st = p.b_k_major ? linear_map(&maps.b, dtype, d_B, K, N, p.k_elems, cols_b) : linear_map(&maps.b, dtype, d_B, N, K, 64, 64);
+    if (st) return st;
+
+    if (choice.pair_nb) {
+        st = linear_map(&maps.c, out_dtype, d_C, N, M, 64, 32);
+        if (!st && d_residual) st = linear_map(&maps.residual, out_dtype, d_residual, N, M, 64, 32);
+        if (!st && d_pre) st = linear_map(&maps.pre, out_dtype, d_pre, N, M, 64, 32);
+        if (st) return st;
+        p.tiles_m = ceil_div(M, 256);
+        p.tiles_n = ceil_div(N, choice.pair_nb);
+        if ((long)p.tiles_m * p.tiles_n > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
+        p.num_tiles = p.tiles_m * p.tiles_n;
+        const int pairs = std::max(1, std::min(sms / 2, p.num_tiles));
+        auto go = [&](auto kernel, int smem) -> int {
+            ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)smem, stream, maps, p));
+            return ESMM_OK;
+        };
+        if (choice.pair_nb == 256)
+            return f8 ? go(esmm_linear_pair_kernel<256, true>, LinearPairCfg<256>::SMEM) : go(esmm_linear_pair_kernel<256, false>, LinearPairCfg<256>::SMEM);
+        return f8 ? go(esmm_linear_pair_kernel<128, true>, LinearPairCfg<128>::SMEM) : go(esmm_linear_pair_kernel<128, false>, LinearPairCfg<128>::SMEM);
+    }
+
+    p.tiles_m = ceil_div(M, 128);
+    p.tiles_n = ceil_div(N, choice.nb);
+    if ((long)p.tiles_m * p.tiles_n * choice.split > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
+    p.num_tiles = p.tiles_m * p.tiles_n;
+    p.a_stage_bytes = a_box_rows * L_KBYTES;
+    const int b_stage = choice.nb * L_KBYTES, steps = ceil_div(p.ksteps, choice.split);
+    // two CTAs per SM; the MMA reads 128 rows of A from any slot, so past the last one the B ring (16 KB at least) has to follow
+    p.stages = std::min({LS_MAX_STAGES, steps, (112 * 1024 - 512) / (p.a_stage_bytes + b_stage)});
+    p.stages = std::max(p.stages, ceil_div(128 * L_KBYTES, b_stage));
+    const int ring = p.stages * (p.a_stage_bytes + b_stage);
+    const int bar_off = (std::max(ring, ls_red_bytes(std::min(M, 128), choice.nb)) + 15) & ~15;
+    const size_t smem = (size_t)bar_off + (2 * LS_MAX_STAGES + 1) * 8 + 16;
+    if (smem > (size_t)SMEM_LIMIT) return ESMM_ERR_TOO_LARGE;
+    auto go = [&](auto kernel) -> int {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(p.num_tiles * choice.split));
+        cfg.blockDim = dim3(LS_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)choice.split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = tuning_get("NO_DEPENDENT_LAUNCH", 0) ? 1 : 2;
+        ESMM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, p, choice.split, bar_off));
+        return ESMM_OK;
+    };
+    if (choice.nb == 64) return f8 ? go(esmm_linear_split_kernel<64, true>) : go(esmm_linear_split_kernel<64, false>);
+    return f8 ? go(esmm_linear_split_kernel<128, true>) : go(esmm_linear_split_kernel<128, false>);
+}

@@ -231,7 +231,7 @@ int esmm_selftest_bounded_wait(unsigned budget_us, void *stream);
  * Names: TILE_M (64 | 128), STAGES, BROW_BITS, ROW_DENSITY, FORCE_LISTED, NO_RUN_TILES, VEC_PATTERNS
  * (0 | 4 | 16), NO_SKINNY, SKINNY_ROWS (16 | 32), PRODUCER_WARPS (3 | 7 | 0: pins the tiled kernel's launch shape),
  * BLOCK_MODE (0 | 1: pins the tiled kernel's way of working, see esmm_gemm_blocks.cuh; -1: its own rule, also in short launches), NO_DEPENDENT_LAUNCH, GROUP_M, GRID, TF32_PAIR (0 | 128 | 256), TF32_SPLIT_LAST,
- * TF32_DIRECT_STORES, and SWIZZLE and PACK, which are accepted and without effect (the kernels they were for are gone).  esmm_tuning_set returns ESMM_ERR_UNSUPPORTED for any other name;
+ * TF32_DIRECT_STORES, LINEAR_PAIR (0 | 128 | 256), LINEAR_SPLIT (1 .. 8) and LINEAR_COLUMNS (64 | 128), which pin esmm_linear's kernel, parts of K and tile width, and SWIZZLE and PACK, which are accepted and without effect (the kernels they were for are gone).  esmm_tuning_set returns ESMM_ERR_UNSUPPORTED for any other name;
  * esmm_tuning_reset returns every hook to "unset" (the library's own choice).
  */
 int esmm_tuning_set(const char *name, int value);
@@ -301,6 +301,101 @@ int esmm_tf32x3_b_live_k(const esmm_tf32x3_b *b);
 size_t esmm_tf32x3_workspace_bytes(int M, int K);
 int esmm_sgemm_joint_tf32x3(int M, const float *d_A, const esmm_tf32x3_b *b, float *d_C, void *d_workspace,
                             void *stream);
+
+/* ---- dense operators around a layer's products ------------------------------ */
+
+/*
+ * What a feed-forward layer does beside its joint-sparse products: the norm before it, products in 16 and 8 bits with
+ * everything that follows them in their epilogue, and the gradients of both.  No counterpart in the reference.
+ * Matrices are dense row-major as everywhere; d_ pointers are device pointers of the element type that the call names:
+ */
+typedef enum esmm_dtype {
+    ESMM_F32 = 0,
+    ESMM_F16 = 1,
+    ESMM_BF16 = 2,
+    ESMM_E4M3 = 3             /* 8-bit floats, 4 bits of exponent and 3 of mantissa, largest value 448; held with FP32 scales */
+} esmm_dtype;
+
+/* gelu is z / 2 (1 + erf(z / sqrt 2)), gelu_tanh z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), silu z / (1 + exp(-z)) */
+typedef enum esmm_activation {
+    ESMM_ACT_NONE = 0,
+    ESMM_ACT_RELU = 1,
+    ESMM_ACT_GELU = 2,
+    ESMM_ACT_GELU_TANH = 3,
+    ESMM_ACT_SILU = 4
+} esmm_activation;
+
+/*
+ * Root-mean-square norm of M rows of K values with the residual's addition:
+ *   h = x + residual,  rstd_i = 1 / sqrt(mean_k h_ik^2 + eps),  y_ik = h_ik rstd_i weight_k
+ * in 32 bits, from the unrounded h.  dtype (ESMM_F32, ESMM_F16, ESMM_BF16) is the type of x, residual, weight and sum.
+ *   d_residual  M x K or NULL (h = x);  d_weight  K or NULL (ones)
+ *   d_sum       M x K or NULL: h, rounded once; may be d_x or d_residual itself (the residual stream, updated in place)
+ *   out_dtype   dtype: d_out gets y, rounded once.  ESMM_E4M3: d_scale[i] = max(amax_k |y_ik|, 2^-100) / 448 and d_out gets
+ *               y_ik / d_scale[i] in e4m3 (NaN becomes the NaN code and does not count for amax)
+ *   d_out       M x K; may be d_x where the types agree
+ *   d_scale     M floats, read only with ESMM_E4M3 (then required);  d_rstd  M floats or NULL, kept for the backward pass
+ * Any K.  Rows of whole 16-byte vectors in 16-byte aligned buffers are the fast case; others only need their elements' alignment.
+ */
+int esmm_rmsnorm(int M, int K, int dtype, const void *d_x, const void *d_residual, const void *d_weight, float eps, void *d_sum,
+                 int out_dtype, void *d_out, float *d_scale, float *d_rstd, void *stream);
+
+/*
+ * Gradients of esmm_rmsnorm: with xhat = h rstd and g = dout weight,
+ *   dx_ik = rstd_i (g_ik - xhat_ik mean_k(g_ik xhat_ik)) + dsum_ik,   dweight_k = sum_i dout_ik xhat_ik.
+ * dx is the gradient of h, that is of x and of residual alike.
+ *   d_h        what the norm was of: its d_sum, or its d_x where there was no residual;  d_rstd  as the forward pass left it
+ *   d_dsum     M x K gradient that arrives at h beside the norm (along the residual stream), or NULL
+ *   d_dx       M x K; may be d_dout or d_dsum;  d_dweight  K values of dtype, rounded once from 32-bit sums, or NULL
+ *   d_workspace  esmm_rmsnorm_backward_workspace_bytes(M, K) bytes, 16-byte aligned; needed with d_dweight
+ * The sums' order is fixed: equal calls give equal bits.
+ */
+size_t esmm_rmsnorm_backward_workspace_bytes(int M, int K);
+int esmm_rmsnorm_backward(int M, int K, int dtype, const void *d_dout, const void *d_h, const void *d_weight, const float *d_rstd,
+                          const void *d_dsum, void *d_dx, void *d_dweight, void *d_workspace, void *stream);
+
+/*
+ * Rows in e4m3 with one scale each, as esmm_rmsnorm writes them: d_scale[i] = max(amax_k |x_ik|, 2^-100) / 448, d_out = x / scale.
+ * (Between two 8-bit products: the first one's C becomes the second one's A.)
+ */
+int esmm_quantize_rows(int M, int K, int dtype, const void *d_x, void *d_out, float *d_scale, void *stream);
+/*
+ * "B offline" for 8-bit products: B (K x N of dtype, row-major) as N x K e4m3 in d_bt, with one scale per column of B,
+ * d_scale[j] = max(amax_k |B_kj|, 2^-100) / 448.  K % 16 == 0; d_bt 16-byte aligned, N * K bytes; d_scale N floats.
+ */
+int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float *d_scale, void *stream);
+
+/*
+ * Matrix product with its epilogue, on the tensor cores (tcgen05, FP32 accumulation, one rounding):
+ *   Z = a_scale_i b_scale_j sum_k op(A)_ik op(B)_kj + bias_j,   pre = Z,   C = act(Z) + residual.
+ *   dtype       ESMM_F16, ESMM_BF16 or ESMM_E4M3: type of A and B
+ *   trans_a     0: A is M x K.  1: d_A is K x M, its transpose (16-bit types)
+ *   trans_b     0: B is K x N (16-bit types).  1: d_B is N x K, its transpose
+ *   out_dtype   type of C, bias, residual and pre: dtype, or ESMM_F16 / ESMM_BF16 for e4m3 operands
+ *   d_C         M x N, overwritten; not A or B
+ *   d_a_scale   M floats or NULL (ones);  d_b_scale  N floats or NULL (ones)
+ *   d_bias      N values or NULL;  d_residual  M x N or NULL, may be d_C;  d_pre  M x N or NULL (kept for the backward pass)
+ * so a layer's gradients are calls of it: dA = dZ B^T (trans_b = 1 on the forward pass's B), dB = A^T dZ (trans_a = 1).
+ * trans_a with trans_b, and e4m3 operands other than trans_a = 0, trans_b = 1, are ESMM_ERR_UNSUPPORTED.
+ * N % 8 == 0; the stored rows of A and B are whole 16-byte vectors (K, M or N a multiple of 8, K of 16 for e4m3), else
+ * ESMM_ERR_SHAPE.  Matrices, bias, residual and pre are 16-byte aligned.  Any M >= 1 otherwise: few rows, or few tiles of C, are
+ * taken by a kernel that splits K over a thread-block cluster.  No workspace, no atomics: equal calls give equal bits.  The first call on a
+ * device sets kernel attributes; make it outside stream capture.
+ */
+int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int trans_a, const void *d_B, int trans_b, int out_dtype, void *d_C,
+                const float *d_a_scale, const float *d_b_scale, const void *d_bias, const void *d_residual, void *d_pre,
+                int activation, void *stream);
+
+/*
+ * Gradient of a product's epilogue, for esmm_linear (16-bit types) and for FP32 products alike: dZ = dC act'(pre), rounded once, and
+ * dbias_j = sum_i dC_ij act'(pre_ij), from the unrounded products.  (The residual's gradient is dC itself.)
+ *   d_pre    M x N, not read with ESMM_ACT_NONE;  d_dZ  M x N or NULL, may be d_dC;  d_dbias  N values of dtype or NULL; one of both
+ *   d_workspace  esmm_epilogue_backward_workspace_bytes(M, N) bytes, 16-byte aligned; needed with d_dbias
+ * N a multiple of 8 (4 for ESMM_F32), matrices 16-byte aligned.  Equal calls give equal bits.
+ */
+size_t esmm_epilogue_backward_workspace_bytes(int M, int N);
+int esmm_epilogue_backward(int M, int N, int dtype, const void *d_dC, const void *d_pre, int activation, void *d_dZ, void *d_dbias,
+                           void *d_workspace, void *stream);
 
 /* cuSPARSE SpMM baseline (src/benchmarks/cusparse_benchmark.cu:56-247): A (M x K, row-major, dense
  * storage) is converted to CSR and multiplied with dense B into C.  *spmm_ms: average of `runs` SpMM

@@ -1,0 +1,257 @@
+"""GPU tests of esmm_linear and esmm_epilogue_backward against 64-bit products: operand layouts and types, every part of the
+epilogue, ragged and smallest sizes, each of its kernels, streams, graphs, and a layer's gradients."""
+import pytest
+import torch
+
+import dense_ops as d
+
+pytestmark = pytest.mark.gpu
+
+
+def operands(m, n, k, t, trans_a=False, trans_b=False, seed=0, std=1.0):
+    """(A as stored, B as stored, op(A) and op(B) in 64 bits)"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    a = torch.randn((m, k), generator=gen, device="cuda") * std
+    b = torch.randn((k, n), generator=gen, device="cuda") / k ** 0.5
+    a, b = a.to(d.TYPES[t]), b.to(d.TYPES[t])
+    return (a.t().contiguous() if trans_a else a, b.t().contiguous() if trans_b else b, a.double(), b.double())
+
+
+def check(pkg, m, n, k, t, out="", trans_a=False, trans_b=False, activation="none", bias=False, residual=False, pre=False, scales=False,
+          seed=0, stream=0, inplace=False):
+    out = out or t
+    trans_b = trans_b or t == "e4m3"
+    a, b, a64, b64 = operands(m, n, k, t, trans_a, trans_b, seed)
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1)
+    ot = d.TYPES[out]
+    bias_t = torch.randn((n,), generator=gen, device="cuda").to(ot) if bias else None
+    res = torch.randn((m, n), generator=gen, device="cuda").to(ot) if residual else None
+    sa = torch.rand((m,), generator=gen, device="cuda") + 0.5 if scales else None
+    sb = torch.rand((n,), generator=gen, device="cuda") + 0.5 if scales else None
+    c, c_ok = d.guarded(m, n, ot)
+    p, p_ok = d.guarded(m, n, ot)
+    c.fill_(float("nan"))
+    if inplace:
+        c.copy_(res)
+    ptr = lambda x: 0 if x is None else x.data_ptr()  # noqa: E731
+    pkg.linear(m, n, k, d.code(pkg, t), ptr(a), ptr(b), d.code(pkg, out), ptr(c), trans_a=int(trans_a), trans_b=int(trans_b), a_scale=ptr(sa),
+               b_scale=ptr(sb), bias=ptr(bias_t), residual=ptr(c if inplace else res), pre=ptr(p) if pre else 0,
+               activation=d.act_code(pkg, activation), stream=stream)
+    pkg.device_status(stream)
+    z, want, mag = d.linear(a64, b64, sa, sb, bias_t, activation, res)
+    u = d.half_step(out)
+    # an activation's slope is at most 1.13; its own arithmetic and the residual's addition are a few 32-bit roundings
+    off = 1.13 * d.sum_error(mag, k) + 2.0 ** -20 * (z.abs() + want.abs())
+    d.assert_close(c, want, off + u * (want.abs() + off) + d.smallest(out), "C")
+    if pre:
+        d.assert_close(p, z, d.sum_error(mag, k) + u * (z.abs() + d.sum_error(mag, k)) + d.smallest(out), "pre")
+    assert c_ok() and p_ok()
+    return c
+
+
+SIZES = [(1, 8, 16), (1, 128, 64), (7, 200, 48), (16, 520, 1040), (33, 72, 256), (127, 136, 2000), (128, 128, 128), (129, 264, 80), (300, 392, 528),
+         (513, 1032, 336)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("t", ["bf16", "f16", "e4m3"])
+def test_sizes(cuda, pkg, t, m, n, k):
+    check(pkg, m, n, k, t, out="bf16" if t == "e4m3" else t)
+    check(pkg, m, n, k, t, out="f16" if t == "e4m3" else t, activation="silu", bias=True, residual=True, pre=True, scales=True, seed=3)
+
+
+@pytest.mark.parametrize("pair", [0, 128, 256])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 8), (40, 72, 72), (256, 256, 64), (264, 520, 200), (1000, 1512, 328)])
+@pytest.mark.parametrize("trans", ["nn", "nt", "tn"])
+def test_kernels_and_layouts(cuda, pkg, tuning, pair, m, n, k, trans):
+    if trans == "tn":
+        m = -(-m // 8) * 8
+    tuning("LINEAR_PAIR", pair)
+    for t in ("bf16", "f16"):
+        check(pkg, m, n, k, t, trans_a=trans == "tn", trans_b=trans == "nt", activation="gelu", bias=True, residual=True, pre=True)
+
+
+@pytest.mark.parametrize("pair", [0, 128, 256])
+def test_e4m3_kernels(cuda, pkg, tuning, pair):
+    tuning("LINEAR_PAIR", pair)
+    for (m, n, k) in [(1, 8, 16), (264, 520, 400), (700, 776, 1168)]:
+        check(pkg, m, n, k, "e4m3", out="bf16", activation="gelu_tanh", bias=True, residual=True, pre=True, scales=True)
+
+
+@pytest.mark.parametrize("split", [1, 2, 3, 8])
+@pytest.mark.parametrize("columns", [64, 128])
+def test_parts_of_k(cuda, pkg, tuning, split, columns):
+    tuning("LINEAR_PAIR", 0)
+    tuning("LINEAR_SPLIT", split)
+    tuning("LINEAR_COLUMNS", columns)
+    for t, (m, n, k) in [("bf16", (5, 136, 1000)), ("bf16", (200, 264, 72)), ("e4m3", (130, 72, 2064)), ("f16", (128, 320, 640))]:
+        check(pkg, m, n, k, t, out="bf16" if t == "e4m3" else t, bias=True, residual=True, scales=True)
+
+
+@pytest.mark.parametrize("activation", d.ACTS)
+@pytest.mark.parametrize("pair", [0, 256])
+def test_epilogue_parts(cuda, pkg, tuning, activation, pair):
+    tuning("LINEAR_PAIR", pair)
+    for bits in range(16):
+        check(pkg, 130, 200, 96, "bf16", activation=activation, bias=bool(bits & 1), residual=bool(bits & 2), pre=bool(bits & 4), scales=bool(bits & 8),
+              seed=bits)
+
+
+@pytest.mark.parametrize("pair", [0, 128, 256])
+def test_residual_in_place(cuda, pkg, tuning, pair):
+    tuning("LINEAR_PAIR", pair)
+    check(pkg, 300, 328, 128, "f16", bias=True, residual=True, inplace=True, activation="relu")
+
+
+def test_long_k_and_many_tiles(cuda, pkg):
+    check(pkg, 16, 256, 16384, "bf16")
+    check(pkg, 2100, 4104, 512, "bf16", bias=True, activation="silu", residual=True)
+    check(pkg, 4096, 2048, 2048, "e4m3", out="bf16", scales=True)
+
+
+@pytest.mark.parametrize("pair", [0, 256])
+def test_infinities_and_nan_stay_in_their_rows_and_columns(cuda, pkg, tuning, pair):
+    tuning("LINEAR_PAIR", pair)
+    m, n, k = 40, 72, 136
+    a, b, _, _ = operands(m, n, k, "bf16")
+    a[3, 5], a[7, 9], b[11, 13] = float("nan"), float("inf"), float("inf")
+    for activation in ("none", "relu"):
+        c = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+        pkg.linear(m, n, k, pkg.BF16, a.data_ptr(), b.data_ptr(), pkg.BF16, c.data_ptr(), activation=d.act_code(pkg, activation))
+        pkg.device_status()
+        want = d.act(a.double() @ b.double(), activation)
+        assert torch.equal(torch.isnan(c), torch.isnan(want)) and torch.equal(torch.isinf(c), torch.isinf(want))
+
+
+def test_repeats_are_bit_identical(cuda, pkg, tuning):
+    for pair, (m, n, k) in [(0, (16, 1032, 4096)), (0, (300, 264, 1024)), (256, (700, 1032, 512))]:
+        tuning("LINEAR_PAIR", pair)
+        first = check(pkg, m, n, k, "bf16", bias=True, residual=True)
+        for _ in range(3):
+            assert torch.equal(first, check(pkg, m, n, k, "bf16", bias=True, residual=True))
+
+
+def layer_calls(pkg, s, stream):
+    """A layer's training step: product with epilogue, its gradient, the two products of the backward pass."""
+    m, n, k = s["m"], s["n"], s["k"]
+    ptr = lambda key: s[key].data_ptr()  # noqa: E731
+    pkg.linear(m, n, k, pkg.BF16, ptr("a"), ptr("b"), pkg.BF16, ptr("c"), bias=ptr("bias"), residual=ptr("residual"), pre=ptr("pre"),
+               activation=pkg.ACT_GELU_TANH, stream=stream)
+    pkg.epilogue_backward(m, n, pkg.BF16, ptr("dc"), ptr("pre"), pkg.ACT_GELU_TANH, ptr("dz"), ptr("dbias"), ptr("ws"), stream)
+    pkg.linear(m, k, n, pkg.BF16, ptr("dz"), ptr("b"), pkg.BF16, ptr("da"), trans_b=1, stream=stream)
+    pkg.linear(k, n, m, pkg.BF16, ptr("a"), ptr("dz"), pkg.BF16, ptr("db"), trans_a=1, stream=stream)
+
+
+def layer_state(pkg, m, n, k, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    normal = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()  # noqa: E731
+    empty = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    return {"m": m, "n": n, "k": k, "a": normal(m, k), "b": (normal(k, n).float() / k ** 0.5).bfloat16(), "bias": normal(n), "residual": normal(m, n),
+            "dc": normal(m, n), "c": empty(m, n), "pre": empty(m, n), "dz": empty(m, n), "dbias": empty(n), "da": empty(m, k), "db": empty(k, n),
+            "ws": torch.empty(pkg.epilogue_backward_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")}
+
+
+def layer_check(s):
+    m, n, k = s["m"], s["n"], s["k"]
+    u, a, b = d.half_step("bf16"), s["a"].double(), s["b"].double()
+    dz = s["dc"].double() * d.act_grad(s["pre"].double(), "gelu_tanh")
+    slope = 2.0 ** -20 * s["dc"].double().abs() * (1 + s["pre"].double().abs())
+    d.assert_close(s["dz"], dz, u * dz.abs() + slope, "dZ")
+    d.assert_close(s["dbias"], dz.sum(0), u * dz.sum(0).abs() + slope.sum(0) + m * 2.0 ** -24 * dz.abs().sum(0), "dbias")
+    got = s["dz"].double()
+    for key, want, mag, length in (("da", got @ b.t(), got.abs() @ b.abs().t(), n), ("db", a.t() @ got, a.abs().t() @ got.abs(), m)):
+        off = d.sum_error(mag, length)
+        d.assert_close(s[key], want, off + u * (want.abs() + off), key)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 8, 8), (9, 72, 136), (130, 264, 200), (520, 776, 1032)])
+def test_layer_gradients(cuda, pkg, m, n, k):
+    s = layer_state(pkg, m, n, k)
+    if m % 8:      # dB = A^T dZ reads A as it lies, its rows being K long: any number of tokens
+        assert k % 8 == 0
+    layer_calls(pkg, s, 0)
+    pkg.device_status()
+    layer_check(s)
+
+
+def test_layer_captured_and_replayed_on_another_stream(cuda, pkg):
+    s = layer_state(pkg, 264, 520, 392)
+    layer_calls(pkg, s, 0)
+    torch.cuda.synchronize()
+    keys = ("c", "pre", "dz", "dbias", "da", "db")
+    want = {key: s[key].clone() for key in keys}
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        layer_calls(pkg, s, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for key in keys:
+            s[key].fill_(float("nan"))
+        graph.replay()
+    torch.cuda.synchronize()
+    pkg.device_status()
+    for key in keys:
+        assert torch.equal(want[key], s[key]), key
+
+
+def test_two_streams_at_once(cuda, pkg):
+    states = [layer_state(pkg, 300, 520, 264, seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, st in zip(states, streams):
+            layer_calls(pkg, s, st.cuda_stream)
+    torch.cuda.synchronize()
+    pkg.device_status()
+    for s in states:
+        layer_check(s)
+
+
+def test_gradients_against_differences(cuda, pkg):
+    """The slope of <dc, C> along a direction of A, by differences in 64 bits at the values that the layer used."""
+    s = layer_state(pkg, 24, 40, 32)
+    layer_calls(pkg, s, 0)
+    torch.cuda.synchronize()
+    a, b, dc = s["a"].double(), s["b"].double(), s["dc"].double()
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    f = lambda x, w: (dc * d.act(x @ w + s["bias"].double(), "gelu_tanh")).sum()  # noqa: E731
+    for key, at in (("da", a), ("db", b)):
+        v = torch.randn(at.shape, generator=gen, device="cuda").double()
+        h = 1e-5
+        slope = (f(a + h * v, b) - f(a - h * v, b) if key == "da" else f(a, b + h * v) - f(a, b - h * v)) / (2 * h)
+        got = (s[key].double() * v).sum()
+        # bf16 roundings of pre, dZ and the gradient itself, each of half a step (of pre: times a second derivative of at most 1.2
+        # and |pre| up to about 5), against the sum of magnitudes
+        dz = s["dz"].double().abs()
+        mag = (dz @ b.abs().t() * v.abs()).sum() if key == "da" else (a.abs().t() @ dz * v.abs()).sum()
+        spread = (dc.abs() * s["pre"].double().abs() * 1.2) @ b.abs().t() if key == "da" else a.abs().t() @ (dc.abs() * s["pre"].double().abs() * 1.2)
+        assert abs(got - slope) <= 2.0 ** -8 * (2 * mag + (spread * v.abs()).sum()), (key, got, slope)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("activation", d.ACTS)
+@pytest.mark.parametrize("m,n", [(1, 8), (9, 264), (1001, 520), (4100, 72)])
+def test_epilogue_backward(cuda, pkg, t, activation, m, n):
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    dc = torch.randn((m, n), generator=gen, device="cuda").to(d.TYPES[t])
+    pre = (3 * torch.randn((m, n), generator=gen, device="cuda")).to(d.TYPES[t])
+    dz, dz_ok = d.guarded(m, n, d.TYPES[t])
+    db, db_ok = d.guarded(1, n, d.TYPES[t])
+    ws = torch.empty(pkg.epilogue_backward_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    pkg.epilogue_backward(m, n, d.code(pkg, t), dc.data_ptr(), pre.data_ptr() if activation != "none" else 0, d.act_code(pkg, activation),
+                          dz.data_ptr(), db.data_ptr(), ws.data_ptr())
+    pkg.device_status()
+    want = dc.double() * d.act_grad(pre.double(), activation)
+    # the slope: an exponential of up to 15 bits of argument, a quotient and a few 32-bit products
+    off = 2.0 ** -20 * dc.double().abs() * (1 + pre.double().abs())
+    u = d.half_step(t)
+    d.assert_close(dz, want, u * want.abs() + off + d.smallest(t), "dZ")
+    total = want.sum(0)
+    d.assert_close(db[0], total, u * total.abs() + off.sum(0) + (m + 40) * 2.0 ** -24 * want.abs().sum(0) + d.smallest(t), "dbias")
+    assert dz_ok() and db_ok()
+    # in place, and each output alone
+    alone = torch.empty_like(db[0])
+    pkg.epilogue_backward(m, n, d.code(pkg, t), dc.data_ptr(), pre.data_ptr(), d.act_code(pkg, activation), 0, alone.data_ptr(), ws.data_ptr())
+    pkg.epilogue_backward(m, n, d.code(pkg, t), dc.data_ptr(), pre.data_ptr(), d.act_code(pkg, activation), dc.data_ptr())
+    pkg.device_status()
+    assert torch.equal(alone, db[0]) and torch.equal(dc, dz)
