@@ -200,6 +200,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return mbar_wait_budget(bar, parity, abort_flag, WAIT_BUDGET_NS);
 }
 
+// After a wait that ran out: what the CTA still has in flight (copies, MMAs) is over long before this is.
+__device__ __forceinline__ void settle_after_timeout()
+{
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
 // 2-D tiled TMA load, completion counted in bytes on an mbarrier of this CTA.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
                                             uint32_t bar)
@@ -219,6 +226,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
         " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+
+// untiled copy: both addresses and the size are multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tma_prefetch_descriptor(const CUtensorMap *map)

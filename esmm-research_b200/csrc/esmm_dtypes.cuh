@@ -64,7 +64,16 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi)
     return r;
 }
 
-__device__ __forceinline__ float e4m3_scale(float amax) { return fmaxf(amax, E4M3_TINY) * (1.0f / E4M3_MAX); }
+__device__ __forceinline__ float e4m3_scale(float amax) { return __fdiv_rn(fmaxf(amax, E4M3_TINY), E4M3_MAX); }
+
+// y / scale from inv = 1 / scale, with the remainder's correction: as good as the division itself, so that values next to a border
+// between two codes fall where the quotient does (a scale that is infinite gives what inv = 0 gives)
+__device__ __forceinline__ float e4m3_quotient(float y, float scale, float inv)
+{
+    const float q = y * inv;
+    const float c = fmaf(fmaf(-q, scale, y), inv, q);
+    return inv > 0.0f ? c : q;
+}
 
 // ---- activations -------------------------------------------------------------------------------------------------
 // silu(z) = z / (1 + exp(-z)).  gelu_tanh(z) = z / 2 (1 + tanh u) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3): one

@@ -9,8 +9,8 @@
 // its gradients (dA = dZ B^T, dB = A^T dZ) need a transposed copy of anything.
 //
 // Two kernels:
-//   esmm_linear_pair_kernel<NB, F8>   large products.  Persistent, a cluster of two CTAs per 256 x NB tile (cta_group::2 MMAs): each CTA
-//       fetches its 128 rows of A and NB / 2 columns of B into a ring, one thread of the even CTA issues the MMAs, eight
+//   esmm_linear_pair_kernel<F8>       large products.  Persistent, a cluster of two CTAs per 256 x 64 .. 256 tile (cta_group::2 MMAs): each CTA
+//       fetches its 128 rows of A and half the columns of B into a ring, one thread of the even CTA issues the MMAs, eight
 //       epilogue warps per CTA drain one of two accumulators in tensor memory while the other is filled.
 //   esmm_linear_split_kernel<NB, F8>  few rows or few tiles: one CTA per 128 x NB tile and part of K, the parts of a tile being one
 //       cluster.  The CTAs add up their accumulators through distributed shared memory in a fixed order, each of them finishing a
@@ -37,6 +37,10 @@ struct LinearParams {
     int a_stage_bytes;                   // split kernel: of A's part of a stage
     uint32_t idesc;
     uint32_t a_lbo, b_lbo;               // leading byte offset of the descriptors, in place
+    uint32_t b_desc_hi;                  // the high word of B's descriptors
+    int b_box_bytes, b_box_cols;         // MN-major B: one of its boxes
+    int nb;                              // pair kernel: columns of a tile
+    int stage_bytes;                     // pair kernel
     uint32_t a_step, b_step;             // from one MMA to the next along K, in 16-byte units
     int bf16;                            // type of C, bias, residual and pre: bfloat16 or float16
     int activation, has_pre, has_residual;
@@ -53,22 +57,48 @@ struct LinearMaps {
 };
 
 constexpr int L_KBYTES = 128;            // bytes of K per step
+// Warps that issue copies, K steps in turn.  (In order of K overall: a step's slot was last used by a step that every earlier wait of the same
+// warp has seen pass, as long as the ring has as many slots as there are such warps.)
+constexpr int L_PRODUCERS = 3;
 constexpr uint32_t L_DESC_HI = 64u | (1u << 14) | (2u << 29);   // eight rows (or k) of 128 bytes every 1024 bytes, version 1, 128-byte swizzle
+constexpr uint32_t L_DESC_HI_64 = 32u | (1u << 14) | (4u << 29);   // eight k of 64 bytes every 512 bytes, 64-byte swizzle
 
 template <bool PAIR, bool F8>
-__device__ __forceinline__ void linear_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate)
+__device__ __forceinline__ void linear_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate)
 {
-#define ESMM_LINEAR_MMA(GROUP, KIND, ZEROS)                                                                            \
+#define ESMM_LINEAR_MMA(GROUP, KIND)                                                                                     \
     asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                         \
-                 "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"                         \
-                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %3, " ZEROS ", p;\n\t}\n" ::"r"(tmem_d), \
-                 "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(L_DESC_HI), "r"(0u)                            \
+                 "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %6};\n\tsetp.ne.b32 p, %4, 0;\n\t"                         \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %3, p;\n\t}\n" ::"r"(tmem_d),             \
+                 "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(L_DESC_HI), "r"(b_hi)                             \
                  : "memory")
-    if constexpr (PAIR && F8) ESMM_LINEAR_MMA("2", "f8f6f4", "{%6, %6, %6, %6, %6, %6, %6, %6}");
-    else if constexpr (PAIR) ESMM_LINEAR_MMA("2", "f16", "{%6, %6, %6, %6, %6, %6, %6, %6}");
-    else if constexpr (F8) ESMM_LINEAR_MMA("1", "f8f6f4", "{%6, %6, %6, %6}");
-    else ESMM_LINEAR_MMA("1", "f16", "{%6, %6, %6, %6}");
+    if constexpr (PAIR && F8) ESMM_LINEAR_MMA("2", "f8f6f4");
+    else if constexpr (PAIR) ESMM_LINEAR_MMA("2", "f16");
+    else if constexpr (F8) ESMM_LINEAR_MMA("1", "f8f6f4");
+    else ESMM_LINEAR_MMA("1", "f16");
 #undef ESMM_LINEAR_MMA
+}
+
+// true in one lane of the warp, the same one every time
+__device__ __forceinline__ bool linear_elect()
+{
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
+    return on != 0;
+}
+
+// The MMAs of one K step by the elected lane.  The loops around it are run by the whole warp, so that the descriptors are computed in
+// uniform registers, where the instruction wants them: from a lane's own branch every MMA took 68 cycles to issue, more
+// than an MMA of 64 columns runs.
+template <bool PAIR, bool F8>
+__device__ __forceinline__ void linear_mma_step(const LinearParams &p, uint32_t d, uint32_t a, uint32_t b, bool more, bool elected)
+{
+    if (elected) {
+        linear_mma<PAIR, F8>(d, a, b, p.b_desc_hi, p.idesc, more ? 1u : 0u);
+#pragma unroll
+        for (uint32_t j = 1; j < 4; ++j) linear_mma<PAIR, F8>(d, a + j * p.a_step, b + j * p.b_step, p.b_desc_hi, p.idesc, 1u);
+    }
+    __syncwarp();
 }
 
 // arrives on the barrier (at this offset in both CTAs of a pair) once the MMAs issued so far are complete
@@ -135,25 +165,23 @@ __device__ __forceinline__ void linear_load(uint32_t dst, const CUtensorMap *map
         tma_load_2d(dst, map, x, y, bar);
 }
 
-// After a wait that ran out: copies and MMAs of this CTA that are still in flight are over long before this is.
-__device__ __forceinline__ void linear_settle()
+__device__ __forceinline__ void linear_prefetch(const CUtensorMap *map, int x, int y)
 {
-    const uint64_t t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 
-// The copies of one K step: lanes 0 .. a_boxes - 1 fetch A, lanes 2 .. 2 + b_boxes - 1 fetch B.  row_a, row_b: first row of op(A) and
+// The copies of one K step: lanes 0 .. a_boxes - 1 fetch A, lanes 4 .. 4 + b_boxes - 1 fetch B.  row_a, row_b: first row of op(A) and
 // column of op(B) of this CTA's part of the tile.
 template <bool PAIR>
 __device__ __forceinline__ void linear_load_step(const LinearParams &p, const LinearMaps &maps, int lane, int step, int row_a, int row_b,
                                                  uint32_t dst_a, uint32_t dst_b, uint32_t bar)
 {
-    const bool is_b = lane >= 2;
-    const int i = lane & 1;
-    if (lane >= 4 || i >= (is_b ? p.b_boxes : p.a_boxes)) return;
-    const int k = step * p.k_elems, r = (is_b ? row_b : row_a) + 64 * i;
+    const bool is_b = lane >= 4;
+    const int i = lane & 3;
+    if (lane >= 8 || i >= (is_b ? p.b_boxes : p.a_boxes)) return;
+    const int k = step * p.k_elems, r = is_b ? row_b + p.b_box_cols * i : row_a + 64 * i;
     const bool k_major = is_b ? p.b_k_major : p.a_k_major;
-    linear_load<PAIR>((is_b ? dst_b : dst_a) + 8192u * (uint32_t)i, is_b ? &maps.b : &maps.a, k_major ? k : r, k_major ? r : k, bar);
+    linear_load<PAIR>(is_b ? dst_b + (uint32_t)(p.b_box_bytes * i) : dst_a + 8192u * (uint32_t)i, is_b ? &maps.b : &maps.a, k_major ? k : r, k_major ? r : k, bar);
 }
 
 // z: 32 sums of one row, columns c0 .. c0 + 31; scale and bias by column in shared memory.
@@ -171,26 +199,21 @@ constexpr int LP_EPI_WARPS = 8;
 constexpr int LP_THREADS = (4 + LP_EPI_WARPS) * 32;
 constexpr int LP_STAGING = 2 * 4096;              // per epilogue warp: two boxes of 32 rows x 64 16-bit columns
 constexpr int LP_MAX_STAGES = 8;
-template <int NB> struct LinearPairCfg {
-    static constexpr int A_BYTES = 128 * L_KBYTES, B_BYTES = (NB / 2) * L_KBYTES;
-    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = NB == 256 ? 5 : 6;
-    static constexpr int RING = STAGES * STAGE_BYTES;
-    static constexpr int STAGING_OFF = RING;
-    static constexpr int COLUMN_OFF = STAGING_OFF + LP_EPI_WARPS * LP_STAGING;   // per epilogue warp: 32 scales, 32 biases
-    static constexpr int BAR_OFF = COLUMN_OFF + LP_EPI_WARPS * 256;
-    static constexpr int SMEM = BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
-    static constexpr int TMEM_COLS = 2 * NB;
-    static_assert(SMEM <= SMEM_LIMIT && STAGES <= LP_MAX_STAGES, "shared memory of a CTA");
-};
+constexpr int LP_MAX_NB = 256;
+constexpr int LP_A_BYTES = 128 * L_KBYTES;
+constexpr int LP_RING = 5 * (LP_A_BYTES + LP_MAX_NB / 2 * L_KBYTES);
+constexpr int LP_COLUMN_OFF = LP_RING + LP_EPI_WARPS * LP_STAGING;       // per epilogue warp: 32 scales, 32 biases
+constexpr int LP_BAR_OFF = LP_COLUMN_OFF + LP_EPI_WARPS * 256;
+constexpr int LP_SMEM = LP_BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
+constexpr int LP_TMEM_COLS = 2 * LP_MAX_NB;
+static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
 
-template <int NB, bool F8>
+template <bool F8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LP_THREADS, 1)
 esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p)
 {
-    using Cfg = LinearPairCfg<NB>;
     extern __shared__ __align__(1024) char smem[];
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::BAR_OFF);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + LP_BAR_OFF);
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + LP_MAX_STAGES), accf0 = smem_u32(bars + 2 * LP_MAX_STAGES),
                    acce0 = smem_u32(bars + 2 * LP_MAX_STAGES + 2), res0 = smem_u32(bars + 2 * LP_MAX_STAGES + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS);
@@ -201,7 +224,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Cfg::STAGES; ++s) {
+        for (int s = 0; s < p.stages; ++s) {
             mbar_init(full0 + 8 * s, 1);                   // (even CTA) its producer; bytes of both CTAs' copies
             mbar_init(empty0 + 8 * s, 1);                  // one commit per stage, delivered to both CTAs
         }
@@ -214,46 +237,51 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
         fence_barrier_init();
         fence_proxy_async();
     }
-    if (warp == 1) {
+    if (warp == L_PRODUCERS) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(Cfg::TMEM_COLS));
+                     "r"(LP_TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
     }
     linear_fence_before();
     __syncthreads();
     linear_cluster_sync();
     linear_fence_after();
+    grid_launch_dependents();
     grid_dependency_wait();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
 
-    if (warp == 0) {
-        // ---------------- producer ----------------
+    if (warp < L_PRODUCERS) {
+        // ---------------- producers: K steps in turn ----------------
         if (lane == 0) tma_prefetch_descriptor(&maps.a);
-        if (lane == 2) tma_prefetch_descriptor(&maps.b);
-        int slot = 0;
+        if (lane == 4) tma_prefetch_descriptor(&maps.b);
+        int slot = warp, first = warp;                     // the slot of this warp's next step, and that step's index in the tile
         uint32_t phase = 0;
         for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
             int tm, tn;
             tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
-            const int row_a = tm * 256 + (int)rank * 128, row_b = tn * NB + (int)rank * (NB / 2);
-            for (int step = 0; step < p.ksteps; ++step) {
+            const int row_a = tm * 256 + (int)rank * 128, row_b = tn * p.nb + (int)rank * (p.nb / 2);
+            int step = first;
+            for (; step < p.ksteps; step += L_PRODUCERS) {
                 ok = mbar_wait(empty0 + 8 * slot, phase ^ 1, abort_flag);
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
-                if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * Cfg::STAGE_BYTES);
+                if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * (uint32_t)p.stage_bytes);
                 __syncwarp();
-                const uint32_t dst = smem_u32(smem) + (uint32_t)slot * Cfg::STAGE_BYTES;
-                linear_load_step<true>(p, maps, lane, step, row_a, row_b, dst, dst + Cfg::A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
-                if (++slot == Cfg::STAGES) {
-                    slot = 0;
+                const uint32_t dst = smem_u32(smem) + (uint32_t)(slot * p.stage_bytes);
+                linear_load_step<true>(p, maps, lane, step, row_a, row_b, dst, dst + LP_A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
+                slot += L_PRODUCERS;
+                if (slot >= p.stages) {
+                    slot -= p.stages;
                     phase ^= 1;
                 }
             }
+            first = step - p.ksteps;
         }
-    } else if (warp == 1) {
+    } else if (warp == L_PRODUCERS) {
         // ---------------- MMA issue: one thread of the even CTA, for both CTAs ----------------
-        if (leader && lane == 0) {
+        if (leader) {
+            const bool elected = linear_elect();
             int slot = 0;
             uint32_t phase = 0, turn = 0;
             bool landed = false;
@@ -261,79 +289,94 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
             for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs, ++turn) {
                 const uint32_t ab = turn & 1u;
                 ok = mbar_wait(acce0 + 8 * ab, ((turn >> 1) & 1u) ^ 1u, abort_flag);   // drained in both CTAs
+                ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 linear_fence_after();
-                const uint32_t d = tmem + ab * (uint32_t)NB;
+                const uint32_t d = tmem + ab * (uint32_t)LP_MAX_NB;
                 for (int step = 0; step < p.ksteps; ++step) {
                     if (!landed) ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
-                    const uint32_t a = (ring + (uint32_t)slot * (Cfg::STAGE_BYTES >> 4)) | p.a_lbo;
-                    const uint32_t b = (ring + (uint32_t)slot * (Cfg::STAGE_BYTES >> 4) + (Cfg::A_BYTES >> 4)) | p.b_lbo;
-                    const int nslot = slot + 1 == Cfg::STAGES ? 0 : slot + 1;
-                    linear_mma<true, F8>(d, a, b, p.idesc, step ? 1u : 0u);
-                    // (a wait costs this thread time even where the data is there: ask while the pipe has work)
+                    const uint32_t at = ring + (uint32_t)(slot * (p.stage_bytes >> 4));
+                    const int nslot = slot + 1 == p.stages ? 0 : slot + 1;
+                    // (a wait costs time even where the data is there: ask for the next step's while this one's MMAs are issued)
                     landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
-#pragma unroll
-                    for (uint32_t j = 1; j < 4; ++j) linear_mma<true, F8>(d, a + j * p.a_step, b + j * p.b_step, p.idesc, 1u);
-                    linear_commit<true>(empty0 + 8 * slot);
-                    if (++slot == Cfg::STAGES) {
+                    linear_mma_step<true, F8>(p, d, at | p.a_lbo, (at + (LP_A_BYTES >> 4)) | p.b_lbo, step != 0, elected);
+                    if (elected) linear_commit<true>(empty0 + 8 * slot);
+                    landed = __all_sync(0xFFFFFFFFu, landed);
+                    if (++slot == p.stages) {
                         slot = 0;
                         phase ^= 1;
                     }
                 }
                 if (!ok) break;
-                linear_commit<true>(accf0 + 8 * ab);
+                if (elected) linear_commit<true>(accf0 + 8 * ab);
+                __syncwarp();
             }
         }
     } else if (warp >= 4) {
         // ---------------- epilogue: a row per thread, 64 columns at a time through the warp's staging boxes ----------------
-        const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns NB / 2 * half ..
-        constexpr int CHUNKS = NB / 128;
-        char *box = smem + Cfg::STAGING_OFF + w * LP_STAGING;
-        float *col_scale = reinterpret_cast<float *>(smem + Cfg::COLUMN_OFF + w * 256), *col_bias = col_scale + 32;
+        const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns 64 (half + 2 c) ..
+        const int chunks = (p.nb / 64 - half + 1) / 2;            // of the tile's 64-column pieces, every other one: none to two
+        constexpr int CHUNKS = 2;
+        char *box = smem + LP_RING + w * LP_STAGING;
+        float *col_scale = reinterpret_cast<float *>(smem + LP_COLUMN_OFF + w * 256), *col_bias = col_scale + 32;
         const uint32_t res_bar = res0 + 8 * w;
         uint32_t turn = 0, res_phase = 0;
         for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs, ++turn) {
             int tm, tn;
             tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
-            const int row0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tn * NB + half * (NB / 2);
+            const int row0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tn * p.nb + half * 64;
             const uint32_t ab = turn & 1u;
+            const bool residual_here = p.has_residual && chunks > 0 && row0 < p.M && col0 < p.N;
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the boxes are free again
-            if (p.has_residual && row0 < p.M && col0 < p.N) {
+            if (residual_here) {
                 if (lane == 0) {
-                    const int boxes = CHUNKS == 2 && col0 + 64 < p.N ? 2 : 1;
+                    const int boxes = chunks == 2 && col0 + 128 < p.N ? 2 : 1;
                     mbar_arrive_expect_tx(res_bar, 4096u * (uint32_t)boxes);
-                    for (int c = 0; c < boxes; ++c) tma_load_2d(smem_u32(box) + 4096u * c, &maps.residual, col0 + 64 * c, row0, res_bar);
+                    for (int c = 0; c < boxes; ++c) tma_load_2d(smem_u32(box) + 4096u * c, &maps.residual, col0 + 128 * c, row0, res_bar);
                 }
             }
             __syncwarp();
+            // the tile's scales and biases, a column of every 32 per lane, under the wait for the accumulator
             const float sa = p.a_scale && row0 + lane < p.M ? p.a_scale[row0 + lane] : 1.0f;
+            float scale_of[2 * CHUNKS], bias_of[2 * CHUNKS];
+#pragma unroll
+            for (int i = 0; i < 2 * CHUNKS; ++i) {
+                const int cj = col0 + (i >> 1) * 128 + (i & 1) * 32 + lane;
+                scale_of[i] = p.b_scale && cj < p.N ? p.b_scale[cj] : 1.0f;
+                bias_of[i] = p.bias && cj < p.N ? (p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[cj])
+                                                          : __half2float(static_cast<const __half *>(p.bias)[cj]))
+                                                : 0.0f;
+            }
             ok = mbar_wait(accf0 + 8 * ab, (turn >> 1) & 1u, abort_flag);
             if (!ok) break;
             linear_fence_after();
-            if (p.has_residual && row0 < p.M && col0 < p.N) {
+            if (chunks == 0) {                                    // (the other four warps do all of a narrow tile)
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(linear_map_to_cta(acce0 + 8 * ab, 0)) : "memory");
+                continue;
+            }
+            if (residual_here) {
                 ok = mbar_wait(res_bar, res_phase, abort_flag);
                 if (!ok) break;
                 res_phase ^= 1u;
             }
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
-                const int col = col0 + 64 * c;
+                if (c >= chunks) break;
+                const int col = col0 + 128 * c;
                 char *mine = box + 4096 * c + lane * 128;
                 uint32_t pre[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float z[32];
-                    const int cj = col + 32 * h + lane;
-                    float b = 0.0f;
-                    if (p.bias && cj < p.N)
-                        b = p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.bias)[cj]) : __half2float(static_cast<const __half *>(p.bias)[cj]);
                     __syncwarp();
-                    col_scale[lane] = p.b_scale && cj < p.N ? p.b_scale[cj] : 1.0f;
-                    col_bias[lane] = b;
+                    col_scale[lane] = scale_of[2 * c + h];
+                    col_bias[lane] = bias_of[2 * c + h];
                     __syncwarp();
-                    linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + ab * (uint32_t)NB + (uint32_t)(half * (NB / 2) + 64 * c + 32 * h), z);
-                    if (c == CHUNKS - 1 && h == 1) {              // the accumulator is read: the next but one tile may have it
+                    linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + ab * (uint32_t)LP_MAX_NB + (uint32_t)(half * 64 + 128 * c + 32 * h), z);
+                    if (c == chunks - 1 && h == 1) {              // the accumulator is read: the next but one tile may have it
                         linear_fence_before();
                         __syncwarp();
                         if (lane == 0)
@@ -405,24 +448,91 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     }
 
     if (!ok) {
-        linear_settle();
+        settle_after_timeout();
         if (lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
     }
     linear_fence_before();
     __syncthreads();
     linear_cluster_sync();        // nothing of the other CTA is touched after this
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS));
+    if (warp == L_PRODUCERS) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(LP_TMEM_COLS));
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------
 // Split kernel
 // ----------------------------------------------------------------------------------------------------------------------------
-constexpr int LS_THREADS = 192;                   // warps 0-3 drain the accumulator, 4 copies, 5 issues the MMAs
+constexpr int LS_DRAIN_WARPS = 8;                 // half the accumulator's columns each; then a warp that copies and one that issues the MMAs
+constexpr int LS_THREADS = (LS_DRAIN_WARPS + L_PRODUCERS + 1) * 32;
 constexpr int LS_MAX_STAGES = 16;
 constexpr int LS_MAX_SPLIT = 8;
 
 // shared memory: ring of A, ring of B (the sums lie over both after the last MMA) | barriers, flags
 __host__ __device__ constexpr int ls_red_bytes(int rows, int nb) { return rows * (nb + 4) * 4; }
+
+// The share of CTA `rank` of a tile's outputs: four columns per thread and row, neighbouring threads on neighbouring columns (reads of
+// the other CTAs' sums move 16 bytes per lane without gaps), a few rows at a time so that their loads are under way together.
+// part_base: the sums in each CTA of the cluster (obtained after the cluster barrier, so that no load from them can be moved before it).
+template <int NB, int SPLIT>
+__device__ __forceinline__ void linear_split_finish(const LinearParams &p, const uint32_t (&part_base)[LS_MAX_SPLIT], int rank, int row0, int col0, int rows)
+{
+    constexpr int LANES = NB / 4, ROWS = LS_THREADS / LANES, U = SPLIT == 1 ? 4 : SPLIT <= 4 ? 2 : 1;
+    const int c = (threadIdx.x % LANES) * 4, col = col0 + c;
+    if (col >= p.N) return;
+    auto unpack2 = [&](uint32_t w) { return p.bf16 ? unpack_bf16(w) : unpack_f16(w); };
+    auto pack2 = [&](float lo, float hi) { return p.bf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); };
+    float bias[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {1.f, 1.f, 1.f, 1.f};
+    if (p.bias) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.bias) + (size_t)col * 2);
+        const float2 f0 = unpack2(w.x), f1 = unpack2(w.y);
+        bias[0] = f0.x, bias[1] = f0.y, bias[2] = f1.x, bias[3] = f1.y;
+    }
+    if (p.b_scale) {   // (aligned to its elements only)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sb[j] = p.b_scale[col + j];
+    }
+    for (int r = rank * ROWS + threadIdx.x / LANES; r < rows; r += SPLIT * ROWS * U) {
+        float4 u[U][SPLIT];
+        uint2 res[U];
+        float sa[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int ri = r + i * SPLIT * ROWS;
+            if (ri >= rows) break;
+#pragma unroll
+            for (int part = 0; part < SPLIT; ++part) {
+                const uint32_t at = part_base[part] + (uint32_t)((ri * (NB + 4) + c) * 4);
+                if constexpr (SPLIT == 1)
+                    asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+                else
+                    asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+            }
+            const size_t off = (size_t)(row0 + ri) * p.N + col;
+            if (p.has_residual) res[i] = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.residual) + off * 2);
+            sa[i] = p.a_scale ? p.a_scale[row0 + ri] : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int ri = r + i * SPLIT * ROWS;
+            if (ri >= rows) break;
+            const size_t off = (size_t)(row0 + ri) * p.N + col;
+            float z[4] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w};
+#pragma unroll
+            for (int part = 1; part < SPLIT; ++part) z[0] += u[i][part].x, z[1] += u[i][part].y, z[2] += u[i][part].z, z[3] += u[i][part].w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] = fmaf(z[j] * sa[i], sb[j], bias[j]);
+            const bool inside = bounds_ok(off + 4 <= (size_t)p.M * p.N, p.status, 64);   // checked build: site 64
+            if (p.has_pre && inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.pre) + off * 2) = make_uint2(pack2(z[0], z[1]), pack2(z[2], z[3]));
+            with_activation(p.activation, [&](auto tag) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
+            });
+            if (p.has_residual) {
+                const float2 f0 = unpack2(res[i].x), f1 = unpack2(res[i].y);
+                z[0] += f0.x, z[1] += f0.y, z[2] += f1.x, z[3] += f1.y;
+            }
+            if (inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.C) + off * 2) = make_uint2(pack2(z[0], z[1]), pack2(z[2], z[3]));
+        }
+    }
+}
 
 template <int NB, bool F8>
 __global__ void __launch_bounds__(LS_THREADS)
@@ -453,21 +563,31 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
         fence_barrier_init();
         fence_proxy_async();
     }
-    if (warp == 5) {
+    if (warp == LS_DRAIN_WARPS + L_PRODUCERS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(NB));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
     linear_fence_before();
     __syncthreads();
     linear_fence_after();
+    grid_launch_dependents();
+    // The first K steps of B are brought into L2 while the kernel before this one finishes (only there: should that kernel write B, what is
+    // read after the wait is what it wrote).
+    if (warp >= LS_DRAIN_WARPS && warp < LS_DRAIN_WARPS + L_PRODUCERS && lane < p.b_boxes) {
+        for (int i = warp - LS_DRAIN_WARPS; i < p.stages && s0 + i < s1; i += L_PRODUCERS) {
+            const int k = (s0 + i) * p.k_elems, r = col0 + p.b_box_cols * lane;
+            linear_prefetch(&maps.b, p.b_k_major ? k : r, p.b_k_major ? r : k);
+        }
+    }
     grid_dependency_wait();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
 
-    if (warp == 4) {
-        int slot = 0;
-        uint32_t phase = 0;
-        for (int step = s0; step < s1; ++step) {
+    if (warp >= LS_DRAIN_WARPS && warp < LS_DRAIN_WARPS + L_PRODUCERS) {
+        const int turn = warp - LS_DRAIN_WARPS;
+        int slot = turn % p.stages;
+        uint32_t phase = (uint32_t)(turn / p.stages) & 1u;
+        for (int step = s0 + turn; step < s1; step += L_PRODUCERS) {
             ok = mbar_wait(empty0 + 8 * slot, phase ^ 1, abort_flag);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
@@ -475,43 +595,48 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             __syncwarp();
             linear_load_step<false>(p, maps, lane, step, row0, col0, a_ring + (uint32_t)(slot * p.a_stage_bytes), b_ring + (uint32_t)(slot * B_BYTES),
                                     full0 + 8 * slot);
+            slot += L_PRODUCERS;
+            if (slot >= p.stages) {
+                slot -= p.stages;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == LS_DRAIN_WARPS + L_PRODUCERS) {
+        const bool elected = linear_elect();
+        int slot = 0;
+        uint32_t phase = 0;
+        bool landed = false;
+        const uint32_t a0 = (a_ring & 0x3FFFFu) >> 4, b0 = (b_ring & 0x3FFFFu) >> 4;
+        for (int step = s0; step < s1; ++step) {
+            if (!landed) ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            const int nslot = slot + 1 == p.stages ? 0 : slot + 1;
+            landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
+            linear_mma_step<false, F8>(p, tmem, (a0 + (uint32_t)(slot * (p.a_stage_bytes >> 4))) | p.a_lbo,
+                                       (b0 + (uint32_t)(slot * (B_BYTES >> 4))) | p.b_lbo, step > s0, elected);
+            if (elected) linear_commit<false>(empty0 + 8 * slot);
+            landed = __all_sync(0xFFFFFFFFu, landed);
             if (++slot == p.stages) {
                 slot = 0;
                 phase ^= 1;
             }
         }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            int slot = 0;
-            uint32_t phase = 0;
-            for (int step = s0; step < s1; ++step) {
-                ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
-                if (!ok) break;
-                const uint32_t a = (((a_ring + (uint32_t)(slot * p.a_stage_bytes)) & 0x3FFFFu) >> 4) | p.a_lbo;
-                const uint32_t b = (((b_ring + (uint32_t)(slot * B_BYTES)) & 0x3FFFFu) >> 4) | p.b_lbo;
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j)
-                    linear_mma<false, F8>(tmem, a + j * p.a_step, b + j * p.b_step, p.idesc, step > s0 || j ? 1u : 0u);
-                linear_commit<false>(empty0 + 8 * slot);
-                if (++slot == p.stages) {
-                    slot = 0;
-                    phase ^= 1;
-                }
-            }
-            if (ok) linear_commit<false>(accf);
-        }
-    } else if (warp < 4) {
+        if (ok && elected) linear_commit<false>(accf);
+        __syncwarp();
+    } else {
         // The sums of the rows that exist, to shared memory: 16 bytes apart beyond their length, so that the stores of eight threads
         // (eight rows) fall on all banks.  The ring is free: every copy has landed and every MMA has read it.
         ok = mbar_wait(accf, 0, abort_flag);
-        if (ok && warp * 32 < rows) {
+        const int q = warp & 3, c0 = (warp >> 2) * (NB / 2);      // TMEM lanes 32 q .., columns c0 ..
+        if (ok && q * 32 < rows) {
             linear_fence_after();
-            float *red = reinterpret_cast<float *>(smem) + (size_t)(warp * 32 + lane) * (NB + 4);
-            const bool mine = warp * 32 + lane < rows;
+            float *red = reinterpret_cast<float *>(smem) + (size_t)(q * 32 + lane) * (NB + 4) + c0;
+            const bool mine = q * 32 + lane < rows;
 #pragma unroll
-            for (int c = 0; c < NB; c += 32) {
+            for (int c = 0; c < NB / 2; c += 32) {
                 float z[32];
-                linear_tmem_ld(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, z);
+                linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(c0 + c), z);
                 if (mine) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(red + c + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
@@ -521,74 +646,29 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
         }
     }
     if (!ok) {
-        linear_settle();
+        settle_after_timeout();
         if (lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
     }
     __syncwarp();
     linear_cluster_sync();       // all parts' sums are in their CTAs' shared memory
 
     // Eight outputs of a row at a time: the parts' sums in the order of K, the epilogue, one 16-byte store.
-    const int groups = rows * (NB / 8);
-    const uint32_t red0 = smem_u32(smem);
-    for (int g = rank * LS_THREADS + threadIdx.x; g < groups; g += split * LS_THREADS) {
-        const int r = g / (NB / 8), c = (g - r * (NB / 8)) * 8, row = row0 + r, col = col0 + c;
-        if (col >= p.N) continue;
-        float z[8];
+    uint32_t part_base[LS_MAX_SPLIT];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = 0.0f;
-        const uint32_t at = red0 + (uint32_t)((r * (NB + 4) + c) * 4);
-        for (int part = 0; part < split; ++part) {
-            const uint32_t from = linear_map_to_cta(at, (uint32_t)part);
-            float4 u, v;
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(from));
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(from + 16));
-            z[0] += u.x, z[1] += u.y, z[2] += u.z, z[3] += u.w;
-            z[4] += v.x, z[5] += v.y, z[6] += v.z, z[7] += v.w;
-        }
-        const size_t off = (size_t)row * p.N + col;
-        auto unpack2 = [&](uint32_t v) { return p.bf16 ? unpack_bf16(v) : unpack_f16(v); };
-        auto pack2 = [&](float lo, float hi) { return p.bf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); };
-        if (p.a_scale) {
-            const float sa = p.a_scale[row];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] *= sa;
-        }
-        if (p.b_scale) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] *= p.b_scale[col + j];
-        }
-        if (p.bias) {
-            const uint4 b = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.bias) + (size_t)col * 2);
-            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2(bw[e]);
-                z[2 * e] += f.x;
-                z[2 * e + 1] += f.y;
-            }
-        }
-        const bool inside = bounds_ok(off + 8 <= (size_t)p.M * p.N, p.status, 64);   // checked build: site 64
-        if (p.has_pre && inside)
-            *reinterpret_cast<uint4 *>(static_cast<char *>(p.pre) + off * 2) = make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7]));
-        with_activation(p.activation, [&](auto tag) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
-        });
-        if (p.has_residual) {
-            const uint4 b = *reinterpret_cast<const uint4 *>(static_cast<const char *>(p.residual) + off * 2);
-            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2(bw[e]);
-                z[2 * e] += f.x;
-                z[2 * e + 1] += f.y;
-            }
-        }
-        if (inside)
-            *reinterpret_cast<uint4 *>(static_cast<char *>(p.C) + off * 2) = make_uint4(pack2(z[0], z[1]), pack2(z[2], z[3]), pack2(z[4], z[5]), pack2(z[6], z[7]));
+    for (int part = 0; part < LS_MAX_SPLIT; ++part)
+        part_base[part] = split == 1 ? smem_u32(smem) : linear_map_to_cta(smem_u32(smem), (uint32_t)min(part, split - 1));
+    switch (split) {
+    case 1: linear_split_finish<NB, 1>(p, part_base, rank, row0, col0, rows); break;
+    case 2: linear_split_finish<NB, 2>(p, part_base, rank, row0, col0, rows); break;
+    case 3: linear_split_finish<NB, 3>(p, part_base, rank, row0, col0, rows); break;
+    case 4: linear_split_finish<NB, 4>(p, part_base, rank, row0, col0, rows); break;
+    case 5: linear_split_finish<NB, 5>(p, part_base, rank, row0, col0, rows); break;
+    case 6: linear_split_finish<NB, 6>(p, part_base, rank, row0, col0, rows); break;
+    case 7: linear_split_finish<NB, 7>(p, part_base, rank, row0, col0, rows); break;
+    default: linear_split_finish<NB, 8>(p, part_base, rank, row0, col0, rows); break;
     }
     linear_cluster_sync();       // (the others may still read this CTA's sums)
-    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB));
+    if (warp == LS_DRAIN_WARPS + L_PRODUCERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB));
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------
@@ -603,10 +683,8 @@ static int linear_prepare(int dev, int *sms)
         int n = 0;
         ESMM_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         auto allow = [](auto kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<256, false>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<256, true>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<128, false>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<128, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, false>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, true>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<128, false>, SMEM_LIMIT));
@@ -617,8 +695,9 @@ static int linear_prepare(int dev, int *sms)
     return ESMM_OK;
 }
 
-// Row-major matrix of `outer` rows x `inner` elements of `dtype`, 128-byte swizzle.
-static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner, long outer, int box_inner, int box_outer)
+// Row-major matrix of `outer` rows x `inner` elements of `dtype`.
+static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner, long outer, int box_inner, int box_outer,
+                      CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B)
 {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return record_cuda_error_text("cuTensorMapEncodeTiled entry point not available");
@@ -631,7 +710,7 @@ static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner,
                                      : dtype == ESMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         char buf[96];
         snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -641,28 +720,42 @@ static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner,
 }
 
 struct LinearChoice {
-    int pair_nb;          // 256, 128: the pair kernel's tile; 0: the split kernel
+    int pair_nb;          // 64, 128, 192, 256: the width of the pair kernel's tiles; 0: the split kernel
     int nb, split;        // split kernel
 };
 
-// Which kernel, by the time per SM that each would take, in K steps of a 128 x 128 tile (64 cycles of MMA per SM at 16 bits).
+// Which kernel, tile width and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
+// shapes (M = 1 .. 2048; K and N from 512 to 11008; 16 and 8 bits, B 0.25 to 90 MB, three sets of operands in turn): what the rule picks takes
+// 1.6 % longer than the best variant on average, 13 % at most.
 static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
 {
-    LinearChoice c;
+    LinearChoice c = {0, 128, 1};
     const int pairs = std::max(1, sms / 2);
-    auto rounds = [](long items, long slots) { return (double)((items + slots - 1) / slots); };
-    // the pair kernel: whole rounds of tiles, and the last tile's epilogue
-    const double t256 = rounds((long)ceil_div(M, 256) * ceil_div(N, 256), pairs) * 2.0 * ksteps + 8.0;
-    const double t128 = rounds((long)ceil_div(M, 256) * ceil_div(N, 128), pairs) * 1.2 * ksteps + 6.0;
-    // the split kernel: parts of K so that all SMs have work
-    c.nb = 128;
-    const long tiles = (long)ceil_div(M, 128) * ceil_div(N, c.nb);
-    c.split = (int)std::max(1L, std::min<long>(LS_MAX_SPLIT, 2L * sms / tiles));
-    c.split = std::min(c.split, std::max(1, ksteps / 4));
-    const double ts = rounds(tiles * c.split, 2L * sms) * 2.6 * (double)ceil_div(ksteps, c.split) + 10.0;
-    c.pair_nb = M <= 128 || ts <= std::min(t256, t128) ? 0 : t256 <= t128 ? 256 : 128;
+    const double hbm = ((double)M + N) * ksteps * L_KBYTES / 6.5e6;            // operands once
+    double best = 1e30;
+    for (int nb = 64; nb <= 256; nb += 64) {
+        const long tiles = (long)ceil_div(M, 256) * ceil_div(N, nb), rounds = (tiles + pairs - 1) / pairs;
+        // a K step: the MMAs, or the copies, which are slower the more SMs copy
+        const double step = std::max(nb * 0.00152, (256 + nb) * (0.000337 + 0.000268 * (double)std::min<long>(tiles, pairs) / pairs));
+        const double t = 4.07 + 0.11 * nb / 64 + std::max(rounds * ksteps * step, hbm) + 1.4 * (rounds - 1);
+        if (t < best) best = t, c.pair_nb = nb;
+    }
+    const int rows = std::min(M, 128), box = ceil_div(rows, 8) * 8;
+    for (int nb = 64; nb <= 128; nb += 64) {
+        const long tiles = (long)ceil_div(M, 128) * ceil_div(N, nb);
+        for (int split : {1, 2, 3, 4, 6, 8}) {
+            if (split > ksteps) break;
+            const long ctas = tiles * split, rounds = (ctas + 2 * sms - 1) / (2 * sms);
+            const int steps = ceil_div(ksteps, split);
+            const double kb = (box + nb) * (L_KBYTES / 1000.0);                // copied per step and CTA
+            const double one = rounds * steps * std::max(0.253, kb / 75.0), all = ctas * steps * kb / 17450.0;
+            const double t = 3.55 + 0.31 * rows * nb / 16384 + std::max({one, all, hbm}) + 1.6 * (rounds - 1) +
+                             (split - 1) * (0.19 + (double)M * N * 4 / 1.9e6);  // sums through distributed shared memory
+            if (t < best) best = t, c = {0, nb, split};
+        }
+    }
     const int forced = tuning_get("LINEAR_PAIR", -1);
-    if (forced == 0 || forced == 128 || forced == 256) c.pair_nb = forced;
+    if (forced == 0 || forced == 64 || forced == 128 || forced == 192 || forced == 256) c.pair_nb = forced;
     const int forced_split = tuning_get("LINEAR_SPLIT", 0);
     if (forced_split >= 1 && forced_split <= LS_MAX_SPLIT) c.split = std::min(forced_split, ksteps);
     const int forced_nb = tuning_get("LINEAR_COLUMNS", 0);
@@ -707,9 +800,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     p.b_k_major = trans_b != 0;
     // K-major: the next MMA's 32 bytes of K lie in the same rows; MN-major: its 16 k are two groups of 1024 bytes on
     p.a_step = p.a_k_major ? 2u : 128u;
-    p.b_step = p.b_k_major ? 2u : 128u;
     p.a_lbo = (p.a_k_major ? 1u : 8192u >> 4) << 16;
-    p.b_lbo = (p.b_k_major ? 1u : 8192u >> 4) << 16;
     p.bf16 = out_dtype == ESMM_BF16;
     p.activation = activation;
     p.has_pre = d_pre != nullptr;
@@ -720,7 +811,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     p.residual = d_residual;
     p.pre = d_pre;
     p.C = d_C;
-    p.group_m = GROUP_M;
+    p.group_m = std::max(1, tuning_get("GROUP_M", GROUP_M));
     p.status = device_status_ptr();
     if (!p.status) return ESMM_ERR_CUDA;
 
@@ -731,7 +822,14 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     int a_box_rows = rows_a;
     if (!choice.pair_nb && p.a_k_major && M < rows_a) a_box_rows = ceil_div(M, 8) * 8;
     p.a_boxes = p.a_k_major ? 1 : rows_a / 64;
-    p.b_boxes = p.b_k_major ? 1 : cols_b / 64;
+    // MN-major B in boxes of 64 columns, or of 32 with the 64-byte swizzle where a CTA's columns are no multiple of 64
+    const bool wide = cols_b % 64 == 0;
+    p.b_box_cols = p.b_k_major ? cols_b : wide ? 64 : 32;
+    p.b_box_bytes = p.b_box_cols * (p.b_k_major ? L_KBYTES : 128);
+    p.b_boxes = cols_b / p.b_box_cols;
+    p.b_desc_hi = p.b_k_major || wide ? L_DESC_HI : L_DESC_HI_64;
+    p.b_step = p.b_k_major ? 2u : wide ? 128u : 64u;
+    p.b_lbo = (p.b_k_major ? 1u : (uint32_t)p.b_box_bytes >> 4) << 16;
     // D = F32; A and B: F16 0, BF16 1, E4M3 0; bits 15, 16: MN-major; N >> 3, M >> 4
     const uint32_t ab_type = dtype == ESMM_BF16 ? 1u : 0u;
     const uint32_t mma_m = choice.pair_nb ? 256u : 128u, mma_n = (uint32_t)(choice.pair_nb ? choice.pair_nb : choice.nb);
@@ -741,7 +839,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     LinearMaps maps;
     memset(&maps, 0, sizeof maps);
     st = p.a_k_major ? linear_map(&maps.a, dtype, d_A, K, M, p.k_elems, a_box_rows) : linear_map(&maps.a, dtype, d_A, M, K, 64, 64);
-    if (!st) st = p.b_k_major ? linear_map(&maps.b, dtype, d_B, K, N, p.k_elems, cols_b) : linear_map(&maps.b, dtype, d_B, N, K, 64, 64);
+    if (!st) st = p.b_k_major ? linear_map(&maps.b, dtype, d_B, K, N, p.k_elems, cols_b) : linear_map(&maps.b, dtype, d_B, N, K, p.b_box_cols, 64, wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (st) return st;
 
     if (choice.pair_nb) {
@@ -754,13 +852,14 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
         if ((long)p.tiles_m * p.tiles_n > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
         p.num_tiles = p.tiles_m * p.tiles_n;
         const int pairs = std::max(1, std::min(sms / 2, p.num_tiles));
-        auto go = [&](auto kernel, int smem) -> int {
-            ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)smem, stream, maps, p));
+        p.nb = choice.pair_nb;
+        p.stage_bytes = LP_A_BYTES + p.nb / 2 * L_KBYTES;
+        p.stages = std::min(LP_MAX_STAGES, LP_RING / p.stage_bytes);
+        auto go = [&](auto kernel) -> int {
+            ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)LP_SMEM, stream, maps, p));
             return ESMM_OK;
         };
-        if (choice.pair_nb == 256)
-            return f8 ? go(esmm_linear_pair_kernel<256, true>, LinearPairCfg<256>::SMEM) : go(esmm_linear_pair_kernel<256, false>, LinearPairCfg<256>::SMEM);
-        return f8 ? go(esmm_linear_pair_kernel<128, true>, LinearPairCfg<128>::SMEM) : go(esmm_linear_pair_kernel<128, false>, LinearPairCfg<128>::SMEM);
+        return f8 ? go(esmm_linear_pair_kernel<true>) : go(esmm_linear_pair_kernel<false>);
     }
 
     p.tiles_m = ceil_div(M, 128);

@@ -16,6 +16,7 @@
 // Rows that are no whole 16-byte vectors (or buffers that do not start on 16 bytes) are accessed element by element by the same
 // kernels; rows longer than a CTA's registers hold go through a form that reads them again from L2 instead.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "esmm_dtypes.cuh"
@@ -139,6 +140,7 @@ template <typename T, int VEC, int NV, bool OUT8, bool NORM>
 __global__ void __launch_bounds__(1024)
 esmm_rmsnorm_kernel(const NormParams p)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float slots[64];
     typedef typename Raw<T, VEC>::type raw_t;
@@ -201,7 +203,7 @@ esmm_rmsnorm_kernel(const NormParams p)
             for (int j = 0; j < VEC; ++j) h[i][j] = h[i][j] * rstd * f[j];
         }
     }
-    float inv = 1.0f;
+    float inv = 1.0f, scale = 1.0f;
     if (OUT8) {
         float amax = 0.0f;
 #pragma unroll
@@ -209,7 +211,7 @@ esmm_rmsnorm_kernel(const NormParams p)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, fabsf(h[i][j]));   // (NaN does not count)
         amax = row_reduce<true>(amax, slots + 32);
-        const float scale = e4m3_scale(amax);
+        scale = e4m3_scale(amax);
         inv = 1.0f / scale;
         if (threadIdx.x == 0) p.scale[row] = scale;
     }
@@ -219,10 +221,152 @@ esmm_rmsnorm_kernel(const NormParams p)
         if (c < p.K && bounds_ok(base + c + VEC <= end, p.status, 61)) {
             if constexpr (OUT8) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) h[i][j] *= inv;
+                for (int j = 0; j < VEC; ++j) h[i][j] = e4m3_quotient(h[i][j], scale, inv);
                 store_e4m3<VEC>(static_cast<uint8_t *>(p.out) + base + c, h[i]);
             } else {
                 store_raw<T, VEC>(static_cast<T *>(p.out) + base + c, h[i]);
+            }
+        }
+    }
+}
+
+// Rows that are no whole vectors, in buffers that start on 16 bytes: a thread takes aligned vectors of the matrix as it lies, which hold the
+// end of the row before and the start of the row after at the row's two ends.  Those elements count for nothing, and such vectors are
+// written element by element (8192 x 1021 of bf16 with a residual, element by element throughout 32.6 us, so 12.4; HBM alone 10.2).
+template <typename T, int VEC, int NV, bool OUT8, bool NORM>
+__global__ void __launch_bounds__(1024)
+esmm_rmsnorm_ragged_kernel(const NormParams p)
+{
+    grid_launch_dependents();
+    grid_dependency_wait();
+    __shared__ float slots[64];
+    typedef typename Raw<T, VEC>::type raw_t;
+    const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (row >= (size_t)p.M) return;              // (a whole warp; one row per CTA never leaves here)
+    const size_t begin = row * (size_t)p.K;
+    const int lead = (int)(begin % VEC);                             // elements of the row before in the first vector
+    const size_t first = begin - lead, left = (size_t)p.M * p.K - first;
+    const T *x = static_cast<const T *>(p.x) + first, *res = static_cast<const T *>(p.residual), *weight = static_cast<const T *>(p.weight);
+    if (res) res += first;
+    // vector i of this thread starts at element off(i) from `first`, which is column off(i) - lead of the row; here(i): it holds some of the
+    // row, whole(i): nothing else; in(i, j): its element j belongs to the row
+    auto off = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * VEC; };
+    auto here = [&](int i) { return off(i) < p.K + lead; };
+    auto whole = [&](int i) { return off(i) >= lead && off(i) + VEC <= p.K + lead; };
+    auto in = [&](int i, int j) { return off(i) + j >= lead && off(i) + j < p.K + lead; };
+    auto loadable = [&](int i) { return (size_t)(off(i) + VEC) <= left; };   // the matrix does not end inside it
+    float h[NV][VEC];
+    float ss = 0.0f;
+    {
+        raw_t xr[NV], rr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (here(i) && loadable(i)) {
+                xr[i] = load_raw<T, VEC>(x + off(i));
+                if (res) rr[i] = load_raw<T, VEC>(res + off(i));
+            }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) h[i][j] = 0.0f;
+            if (!here(i)) continue;
+            if (loadable(i)) {
+                unpack<T, VEC>(xr[i], h[i]);
+                if (res) {
+                    float r[VEC];
+                    unpack<T, VEC>(rr[i], r);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) h[i][j] += r[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (in(i, j)) h[i][j] = to_float<T>(x[off(i) + j]) + (res ? to_float<T>(res[off(i) + j]) : 0.0f);
+            }
+            T *to = static_cast<T *>(p.sum) + first + off(i);
+            if (whole(i)) {
+                if (NORM && p.sum) store_raw<T, VEC>(to, h[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (NORM && p.sum && in(i, j)) to[j] = from_float<T>(h[i][j]);
+                    if (!in(i, j)) h[i][j] = 0.0f;                   // (counts for nothing from here on)
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+        }
+    }
+    if (NORM) {
+        float w[NV][VEC];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) w[i][j] = 1.0f;
+            if (!weight || !here(i)) continue;
+            const T *from = weight + (off(i) - lead);
+            if (whole(i)) {
+                if (VEC == 8 && (lead & 1) == 0) {                   // pairs on their own alignment
+                    const uint32_t *pairs = reinterpret_cast<const uint32_t *>(from);
+#pragma unroll
+                    for (int j = 0; j < VEC; j += 2) {
+                        const float2 f = std::is_same<T, __half>::value ? unpack_f16(pairs[j / 2]) : unpack_bf16(pairs[j / 2]);
+                        w[i][j] = f.x, w[i][j + 1] = f.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) w[i][j] = to_float<T>(from[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (in(i, j)) w[i][j] = to_float<T>(from[j]);
+            }
+        }
+        ss = row_reduce<false>(ss, slots);
+        const float rstd = __frsqrt_rn(ss / (float)p.K + p.eps);
+        if (p.rstd && threadIdx.x == 0) p.rstd[row] = rstd;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) h[i][j] = h[i][j] * rstd * w[i][j];
+    }
+    float inv = 1.0f, scale = 1.0f;
+    if (OUT8) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (here(i)) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, whole(i) || in(i, j) ? fabsf(h[i][j]) : 0.0f);
+            }
+        amax = row_reduce<true>(amax, slots + 32);
+        scale = e4m3_scale(amax);
+        inv = 1.0f / scale;
+        if (threadIdx.x == 0) p.scale[row] = scale;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (!here(i)) continue;
+        if constexpr (OUT8) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) h[i][j] = e4m3_quotient(h[i][j], scale, inv);
+            uint8_t *to = static_cast<uint8_t *>(p.out) + first + off(i);
+            if (whole(i)) {
+                store_e4m3<VEC>(to, h[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (in(i, j)) to[j] = (uint8_t)pack_e4m3(h[i][j], 0.0f);
+            }
+        } else {
+            T *to = static_cast<T *>(p.out) + first + off(i);
+            if (whole(i)) {
+                store_raw<T, VEC>(to, h[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (in(i, j)) to[j] = from_float<T>(h[i][j]);
             }
         }
     }
@@ -234,6 +378,7 @@ template <typename T, bool OUT8, bool NORM>
 __global__ void __launch_bounds__(1024)
 esmm_rmsnorm_long_kernel(const NormParams p)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float slots[64];
     const size_t base = (size_t)blockIdx.x * (size_t)p.K;
@@ -250,19 +395,19 @@ esmm_rmsnorm_long_kernel(const NormParams p)
         if (p.rstd && threadIdx.x == 0) p.rstd[blockIdx.x] = rstd;
     }
     auto y_at = [&](float h, int c) { return NORM ? h * rstd * (weight ? to_float<T>(weight[c]) : 1.0f) : h; };
-    float inv = 1.0f;
+    float inv = 1.0f, scale = 1.0f;
     if (OUT8) {
         float amax = 0.0f;
         for (int c = threadIdx.x; c < p.K; c += blockDim.x) amax = fmaxf(amax, fabsf(y_at(h_at(c), c)));
         amax = row_reduce<true>(amax, slots + 32);
-        const float scale = e4m3_scale(amax);
+        scale = e4m3_scale(amax);
         inv = 1.0f / scale;
         if (threadIdx.x == 0) p.scale[blockIdx.x] = scale;
     }
     for (int c = threadIdx.x; c < p.K; c += blockDim.x) {
         const float h = h_at(c), y = y_at(h, c);
         if (NORM && p.sum) static_cast<T *>(p.sum)[base + c] = from_float<T>(h);
-        if (OUT8) static_cast<uint8_t *>(p.out)[base + c] = (uint8_t)pack_e4m3(y * inv, 0.0f);
+        if (OUT8) static_cast<uint8_t *>(p.out)[base + c] = (uint8_t)pack_e4m3(e4m3_quotient(y, scale, inv), 0.0f);
         else static_cast<T *>(p.out)[base + c] = from_float<T>(y);
     }
 }
@@ -274,20 +419,59 @@ struct NormGradParams {
     const float *rstd;
     void *dx;
     float *partial;      // one row of K sums per CTA
+    int stages, row_bytes;
     int *status;
 };
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(1024)
+// The rows come as bulk copies into a ring of `stages` rows of dout, h and dsum, some rows ahead: what is under way does not depend
+// on the registers of the threads that wait for a row's reduction.  A row that does not start on 16 bytes is copied from the boundary before
+// it to the one after it (VEC = 1: its elements are then read one by one); where the matrix ends in between, the last elements are read
+// from where they lie.  KEEP: a thread keeps its part of a row between the row's two passes, and the row's slot is free at once; for the
+// longest rows it reads the slot again.  8192 x 4096 of bf16, without dw: rows through registers, one ahead, 54.3 us; so 43.6 (HBM alone 41.0).
+template <typename T, int VEC, int NV, int THREADS, bool KEEP>
+__global__ void __launch_bounds__(THREADS)
 esmm_rmsnorm_backward_kernel(const NormGradParams p)
 {
-    grid_dependency_wait();
+    extern __shared__ __align__(16) char smem[];   // per group: [stage][dout, h, dsum][row_bytes]; then one barrier per group and stage
     __shared__ float slots[64];
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
     typedef typename Raw<T, VEC>::type raw_t;
+    // blockDim.y groups of blockDim.x threads have a row each (several only where a group is one warp)
+    const int groups = blockDim.y, group = threadIdx.y;
+    const char *ring = smem + (size_t)group * p.stages * 3 * p.row_bytes;
+    const uint32_t ring0 = smem_u32(ring), bars = smem_u32(smem) + (uint32_t)(groups * p.stages * 3 * p.row_bytes + group * p.stages * 8);
     const T *weight = static_cast<const T *>(p.weight);
-    const T *dout = static_cast<const T *>(p.dout), *h = static_cast<const T *>(p.h), *dsum = static_cast<const T *>(p.dsum);
+    const size_t total = (size_t)p.M * p.K * sizeof(T);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) mbar_init(bars + 8 * i, 1);
+        abort_word = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    __syncthreads();
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const bool adds = p.dsum != nullptr;
+    // bytes [lo, hi) of each array are copied for a row
+    auto row_lo = [&](size_t row) { return row * p.K * sizeof(T) & ~(size_t)15; };
+    auto row_hi = [&](size_t row) { return min(((row + 1) * p.K * sizeof(T) + 15) & ~(size_t)15, total & ~(size_t)15); };
+    auto fetch = [&](size_t row, int slot) {
+        const size_t lo = row_lo(row);
+        const uint32_t bytes = (uint32_t)(row_hi(row) - lo), bar = bars + 8 * slot;
+        const uint32_t to = ring0 + (uint32_t)(slot * 3 * p.row_bytes);
+        mbar_arrive_expect_tx(bar, bytes * (adds ? 3u : 2u));
+        if (!bytes) return;
+        bulk_load(to, static_cast<const char *>(p.dout) + lo, bytes, bar);
+        bulk_load(to + (uint32_t)p.row_bytes, static_cast<const char *>(p.h) + lo, bytes, bar);
+        if (adds) bulk_load(to + 2u * (uint32_t)p.row_bytes, static_cast<const char *>(p.dsum) + lo, bytes, bar);
+    };
+    const size_t first = (size_t)blockIdx.x * groups + group, stride = (size_t)gridDim.x * groups;
+    if (threadIdx.x == 0)
+        for (int i = 0; i < p.stages; ++i)
+            if (first + i * stride < (size_t)p.M) fetch(first + i * stride, i);
     float dw[NV][VEC];
-    raw_t w[NV], g_raw[NV], h_raw[NV], s_raw[NV];
+    raw_t w[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * VEC;
@@ -295,69 +479,133 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
         for (int j = 0; j < VEC; ++j) dw[i][j] = 0.0f;
         if (weight && c < p.K) w[i] = load_raw<T, VEC>(weight + c);
     }
-    float rstd_next = 0.0f;
-    auto load_row = [&](size_t row) {
-        const size_t base = row * (size_t)p.K;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < p.K) {
-                g_raw[i] = load_raw<T, VEC>(dout + base + c);
-                h_raw[i] = load_raw<T, VEC>(h + base + c);
-                if (dsum) s_raw[i] = load_raw<T, VEC>(dsum + base + c);
+    bool ok = true;
+    int slot = 0, turn = 0;
+    uint32_t phase = 0;
+    float rstd = first < (size_t)p.M ? p.rstd[first] : 0.0f;
+    for (size_t row = first; row < (size_t)p.M; row += stride, turn ^= 32) {
+        const size_t base = row * (size_t)p.K, next = row + stride;
+        const float rstd_next = next < (size_t)p.M ? p.rstd[next] : 0.0f;
+        const char *g_at = ring + (size_t)slot * 3 * p.row_bytes + (VEC == 1 ? base * sizeof(T) - row_lo(row) : 0);
+        const char *h_at = g_at + p.row_bytes, *s_at = h_at + p.row_bytes;
+        // columns from this one on lie behind what was copied
+        const int copied = VEC == 1 ? (int)min((long long)p.K, ((long long)row_hi(row) - (long long)(base * sizeof(T))) / (long long)sizeof(T)) : p.K;
+        ok = mbar_wait(bars + 8 * slot, phase, abort_flag) && ok;
+        if (VEC == 1 && copied < p.K) {               // the matrix's last elements, to where the copies would have put them
+            for (int c = max(copied, 0) + threadIdx.x; c < p.K; c += blockDim.x) {
+                const uint32_t o = (uint32_t)(slot * 3 * p.row_bytes) + (uint32_t)(base * sizeof(T) - row_lo(row));
+                T *to = reinterpret_cast<T *>(const_cast<char *>(ring) + o) + c;
+                to[0] = static_cast<const T *>(p.dout)[base + c];
+                *reinterpret_cast<T *>(reinterpret_cast<char *>(to) + p.row_bytes) = static_cast<const T *>(p.h)[base + c];
+                if (adds) *reinterpret_cast<T *>(reinterpret_cast<char *>(to) + 2 * p.row_bytes) = static_cast<const T *>(p.dsum)[base + c];
             }
+            if (blockDim.x > 32) __syncthreads();
+            else __syncwarp();
         }
-        rstd_next = p.rstd[row];
-    };
-    load_row(blockIdx.x);
-    int turn = 0;
-    for (size_t row = blockIdx.x; row < (size_t)p.M; row += gridDim.x, turn ^= 32) {
-        const size_t base = row * (size_t)p.K;
-        const float rstd = rstd_next;
-        float gw[NV][VEC], xh[NV][VEC], add[NV][VEC], dot = 0.0f;
+        auto element = [&](const char *at, int c) { return *reinterpret_cast<const raw_t *>(at + (size_t)c * sizeof(T)); };
+        raw_t s_raw[KEEP ? NV : 1];
+        float gw[KEEP ? NV : 1][VEC], xh[KEEP ? NV : 1][VEC], dot[2] = {0.0f, 0.0f};
+        auto products = [&](int i, int c, float (&gwi)[VEC], float (&xhi)[VEC], bool sums) {
+            float f[VEC];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            for (int j = 0; j < VEC; ++j) f[j] = 1.0f;
+            unpack<T, VEC>(element(g_at, c), gwi);
+            unpack<T, VEC>(element(h_at, c), xhi);
+            if (weight) unpack<T, VEC>(w[i], f);
+            if constexpr (VEC == 1) {
+                xhi[0] *= rstd;
+                if (sums) dw[i][0] = fmaf(gwi[0], xhi[0], dw[i][0]);
+                gwi[0] *= f[0];
+                if (sums) dot[0] = fmaf(gwi[0], xhi[0], dot[0]);
+            } else {                                // two at a time
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) gw[i][j] = xh[i][j] = add[i][j] = 0.0f;
-            if (c < p.K) {
-                unpack<T, VEC>(g_raw[i], gw[i]);
-                unpack<T, VEC>(h_raw[i], xh[i]);
-                if (dsum) unpack<T, VEC>(s_raw[i], add[i]);
-                float f[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) f[j] = 1.0f;
-                if (weight) unpack<T, VEC>(w[i], f);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    xh[i][j] *= rstd;
-                    dw[i][j] = fmaf(gw[i][j], xh[i][j], dw[i][j]);
-                    gw[i][j] *= f[j];
-                    dot = fmaf(gw[i][j], xh[i][j], dot);
+                for (int j = 0; j < VEC; j += 2) {
+                    const float2 g2 = make_float2(gwi[j], gwi[j + 1]), x2 = __fmul2_rn(make_float2(xhi[j], xhi[j + 1]), make_float2(rstd, rstd));
+                    const float2 p2 = __fmul2_rn(g2, make_float2(f[j], f[j + 1]));
+                    if (sums) {
+                        const float2 d2 = __ffma2_rn(g2, x2, make_float2(dw[i][j], dw[i][j + 1])), s2 = __ffma2_rn(p2, x2, make_float2(dot[0], dot[1]));
+                        dw[i][j] = d2.x, dw[i][j + 1] = d2.y;
+                        dot[0] = s2.x, dot[1] = s2.y;
+                    }
+                    xhi[j] = x2.x, xhi[j + 1] = x2.y;
+                    gwi[j] = p2.x, gwi[j + 1] = p2.y;
                 }
             }
-        }
-        if (row + gridDim.x < (size_t)p.M) load_row(row + gridDim.x);
-        // (two sets of slots in turn: a warp may be a row ahead of the slowest one's reads)
-        dot = row_reduce<false>(dot, slots + turn) / (float)p.K;
+        };
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < p.K && bounds_ok(base + c + VEC <= (size_t)p.M * p.K, p.status, 62)) {
+            if (c < p.K) {
+                if (KEEP && adds) s_raw[KEEP ? i : 0] = element(s_at, c);
+                products(i, c, gw[KEEP ? i : 0], xh[KEEP ? i : 0], true);
+            }
+        }
+        const float mean = row_reduce<false>(dot[0] + dot[1], slots + turn) / (float)p.K;
+        // every thread has the row in its registers (or, !KEEP, is through with the row before it): that slot takes the next row
+        if (threadIdx.x == 0) {
+            const size_t ahead = row + (KEEP ? p.stages : p.stages - 1) * stride;
+            if (ahead < (size_t)p.M && (KEEP || row != first)) fetch(ahead, KEEP ? slot : slot ? slot - 1 : p.stages - 1);
+        }
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) gw[i][j] = fmaf(rstd, fmaf(-xh[i][j], dot, gw[i][j]), add[i][j]);
-                store_raw<T, VEC>(static_cast<T *>(p.dx) + base + c, gw[i]);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (threadIdx.x + i * blockDim.x) * VEC;
+            if (c < p.K && ok && bounds_ok(base + c + VEC <= (size_t)p.M * p.K, p.status, 62)) {
+                float add[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) add[j] = 0.0f;
+                const int at = KEEP ? i : 0;
+                if constexpr (KEEP) {
+                    if (adds) unpack<T, VEC>(s_raw[at], add);
+                } else {
+                    if (adds) unpack<T, VEC>(element(s_at, c), add);
+                    products(i, c, gw[0], xh[0], false);
+                }
+                if constexpr (VEC == 1) {
+                    gw[at][0] = fmaf(rstd, fmaf(-mean, xh[at][0], gw[at][0]), add[0]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; j += 2) {
+                        const float2 g2 = __ffma2_rn(make_float2(-mean, -mean), make_float2(xh[at][j], xh[at][j + 1]), make_float2(gw[at][j], gw[at][j + 1]));
+                        const float2 o2 = __ffma2_rn(make_float2(rstd, rstd), g2, make_float2(add[j], add[j + 1]));
+                        gw[at][j] = o2.x, gw[at][j + 1] = o2.y;
+                    }
+                }
+                store_raw<T, VEC>(static_cast<T *>(p.dx) + base + c, gw[at]);
+            }
+        }
+        rstd = rstd_next;
+        if (++slot == p.stages) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+    if (!ok) {
+        settle_after_timeout();
+        if ((threadIdx.x & 31) == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
+    }
+    if (!p.partial) return;
+    float *to = p.partial + (size_t)blockIdx.x * p.K;
+    float *mine = groups == 1 ? to : reinterpret_cast<float *>(smem) + (size_t)group * (blockDim.x * NV * VEC);
+    if (groups > 1) __syncthreads();               // (every group's rows are through: the rings' memory is free)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (threadIdx.x + i * blockDim.x) * VEC;
+        if (c < p.K) {
+            if constexpr (VEC >= 4) {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4 *>(mine + c + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
+            } else {
+                mine[c] = dw[i][0];
             }
         }
     }
-    if (p.partial) {
-        float *to = p.partial + (size_t)blockIdx.x * p.K;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < p.K)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) to[c + j] = dw[i][j];
+    if (groups > 1) {
+        __syncthreads();
+        const float *all = reinterpret_cast<const float *>(smem);
+        for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < p.K; c += blockDim.x * groups) {
+            float sum = 0.0f;
+            for (int g = 0; g < groups; ++g) sum += all[(size_t)g * (blockDim.x * NV * VEC) + c];
+            to[c] = sum;
         }
     }
 }
@@ -367,6 +615,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
 esmm_rmsnorm_backward_long_kernel(const NormGradParams p)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float slots[64];
     const T *weight = static_cast<const T *>(p.weight);
@@ -390,31 +639,54 @@ esmm_rmsnorm_backward_long_kernel(const NormGradParams p)
     }
 }
 
-// out[c] = sum over `rows` rows of partial[r][c], in a fixed order: 32 columns per CTA, thread row y takes rows y, y + 32, ..., the 32
-// sums are added as a tree.
+// out[c] = sum over `rows` rows of partial[r][c], in a fixed order: 32 columns per CTA, four per thread, thread row y takes rows y, y + 64,
+// ..., the 64 sums are added as a tree.
 template <typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(512)
 esmm_column_sum_kernel(const float *partial, int rows, int K, T *out)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
-    __shared__ float sums[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
-    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-    if (c < K) {
-        const float *at = partial + c;
-        int r = threadIdx.y;
-        for (; r + 96 < rows; r += 128) {
-            s0 += at[(size_t)r * K];
-            s1 += at[(size_t)(r + 32) * K];
-            s2 += at[(size_t)(r + 64) * K];
-            s3 += at[(size_t)(r + 96) * K];
+    __shared__ float sums[64][33];
+    const int c = blockIdx.x * 32 + threadIdx.x * 4;
+    const bool vectors = K % 4 == 0;
+    float4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto take = [&](float4 &sum, int r) {
+        const float *at = partial + (size_t)r * K + c;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (vectors) {
+            if (c < K) v = *reinterpret_cast<const float4 *>(at);
+        } else {
+            if (c < K) v.x = at[0];
+            if (c + 1 < K) v.y = at[1];
+            if (c + 2 < K) v.z = at[2];
+            if (c + 3 < K) v.w = at[3];
         }
-        for (; r < rows; r += 32) s0 += at[(size_t)r * K];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    };
+    int r = threadIdx.y;
+    for (; r + 192 < rows; r += 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take(s[i], r + 64 * i);
     }
-    sums[threadIdx.y][threadIdx.x] = (s0 + s1) + (s2 + s3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (r + 64 * i < rows) take(s[i], r + 64 * i);
+    float *mine = &sums[threadIdx.y][threadIdx.x * 4];
+    mine[0] = (s[0].x + s[1].x) + (s[2].x + s[3].x);
+    mine[1] = (s[0].y + s[1].y) + (s[2].y + s[3].y);
+    mine[2] = (s[0].z + s[1].z) + (s[2].z + s[3].z);
+    mine[3] = (s[0].w + s[1].w) + (s[2].w + s[3].w);
     __syncthreads();
-    const float s = warp_sum(sums[threadIdx.x][threadIdx.y]);   // thread row y adds up column y
-    if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < K) out[blockIdx.x * 32 + threadIdx.y] = from_float<T>(s);
+    const int warp = (threadIdx.y * 8 + threadIdx.x) >> 5, lane = (threadIdx.y * 8 + threadIdx.x) & 31;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                 // a warp adds up two of the 32 columns
+        const int col = warp * 2 + i;
+        const float v = warp_sum(sums[lane][col] + sums[lane + 32][col]);
+        if (lane == 0 && blockIdx.x * 32 + col < K) out[blockIdx.x * 32 + col] = from_float<T>(v);
+    }
 }
 
 // ---- gradient of a product's epilogue --------------------------------------------------------------------------------------
@@ -431,6 +703,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 esmm_epilogue_backward_kernel(const EpiGradParams p)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     constexpr int VEC = 16 / sizeof(T), U = 4;         // rows in flight per warp
     typedef typename Raw<T, VEC>::type raw_t;
@@ -491,6 +764,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
 esmm_column_scale_kernel(const T *B, int K, int N, float *scale)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float part[32][33];
     const int n = blockIdx.x * 32 + threadIdx.x;
@@ -509,13 +783,14 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 esmm_quantize_transpose_kernel(const T *B, int K, int N, const float *scale, uint8_t *bt)
 {
+    grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float tile[128][33];
     const int k0 = blockIdx.y * 128, n0 = blockIdx.x * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float inv = n0 + lane < N ? 1.0f / scale[n0 + lane] : 0.0f;
+    const float sc = n0 + lane < N ? scale[n0 + lane] : 1.0f, inv = 1.0f / sc;
     for (int r = warp; r < 128; r += 8)
-        tile[r][lane] = k0 + r < K && n0 + lane < N ? to_float<T>(B[(size_t)(k0 + r) * N + n0 + lane]) * inv : 0.0f;
+        tile[r][lane] = k0 + r < K && n0 + lane < N ? e4m3_quotient(to_float<T>(B[(size_t)(k0 + r) * N + n0 + lane]), sc, inv) : 0.0f;
     __syncthreads();
     for (int c = warp; c < 32; c += 8) {
         const int n = n0 + c, k = k0 + lane * 4;
@@ -540,91 +815,131 @@ constexpr int NORM_ROWS_PER_SM = 8;
 
 static int sm_count(int *sms)
 {
+    static std::atomic<int> known[64];
     int dev = 0;
     ESMM_CUDA_TRY(cudaGetDevice(&dev));
-    ESMM_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    int n = dev >= 0 && dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (!n) {
+        ESMM_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
     return ESMM_OK;
 }
 
 template <typename T, bool OUT8, bool NORM>
-static int norm_launch_type(const NormParams &p, bool vectors, int sms, cudaStream_t stream)
+static int norm_launch_type(const NormParams &p, bool aligned, int sms, cudaStream_t stream)
 {
     constexpr int VEC = 16 / (int)sizeof(T);
-    const bool many = (long)p.M > (long)NORM_ROWS_PER_SM * sms;
-    auto go = [&](auto kernel, int vec, int nv) -> int {
-        const int warps = ceil_div(ceil_div(p.K, vec * nv), 32);
+    const bool many = (long)p.M > (long)NORM_ROWS_PER_SM * sms, vectors = aligned && p.K % VEC == 0;
+    // a vector's worth of elements for every `nv`-th thread and its row
+    auto go = [&](auto kernel, int units, int nv) -> int {
+        const int warps = ceil_div(ceil_div(units, nv), 32);
         const int rows = warps == 1 ? 8 : 1;
         ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)ceil_div(p.M, rows)), dim3(warps * 32, rows), 0, stream, p));
         return ESMM_OK;
     };
-    const int units = vectors ? ceil_div(p.K, VEC) : p.K;
-    if (vectors) {
-        if (units > 1024 * 4 || (many && units > 32 * 2)) {
-            if (units <= 1024 * 4) return go(esmm_rmsnorm_kernel<T, VEC, 4, OUT8, NORM>, VEC, 4);
-        } else {
-            if (units <= (many ? 32 : 1024)) return go(esmm_rmsnorm_kernel<T, VEC, 1, OUT8, NORM>, VEC, 1);
-            if (units <= 1024 * 2) return go(esmm_rmsnorm_kernel<T, VEC, 2, OUT8, NORM>, VEC, 2);
-            return go(esmm_rmsnorm_kernel<T, VEC, 4, OUT8, NORM>, VEC, 4);
-        }
-    } else {
-        if (units <= 32 * 4 || (!many && units <= 1024 * 4)) return go(esmm_rmsnorm_kernel<T, 1, 4, OUT8, NORM>, 1, 4);
-        if (units <= 1024 * 16) return go(esmm_rmsnorm_kernel<T, 1, 16, OUT8, NORM>, 1, 16);
-    }
+    const int units = vectors ? p.K / VEC : aligned ? p.K / VEC + 2 : p.K;
+    const int nv = units <= (many ? 32 : 1024) ? 1 : units <= (many ? 64 : 2048) ? 2 : 4;
+    if (vectors && units <= 4096)
+        return nv == 1   ? go(esmm_rmsnorm_kernel<T, VEC, 1, OUT8, NORM>, units, 1)
+               : nv == 2 ? go(esmm_rmsnorm_kernel<T, VEC, 2, OUT8, NORM>, units, 2)
+                         : go(esmm_rmsnorm_kernel<T, VEC, 4, OUT8, NORM>, units, 4);
+    if (!vectors && aligned && units <= 2048)
+        return units <= (many ? 32 : 1024) ? go(esmm_rmsnorm_ragged_kernel<T, VEC, 1, OUT8, NORM>, units, 1)
+                                           : go(esmm_rmsnorm_ragged_kernel<T, VEC, 2, OUT8, NORM>, units, 2);
+    if (!aligned && units <= 4096) return go(esmm_rmsnorm_kernel<T, 1, 4, OUT8, NORM>, units, 4);
     ESMM_CUDA_TRY(launch_dependent(esmm_rmsnorm_long_kernel<T, OUT8, NORM>, dim3((unsigned)p.M), dim3(1024), 0, stream, p));
     return ESMM_OK;
 }
 
 template <bool NORM>
-static int norm_launch(const NormParams &p, int dtype, bool out8, bool vectors, cudaStream_t stream)
+static int norm_launch(const NormParams &p, int dtype, bool out8, bool aligned, cudaStream_t stream)
 {
     int sms = 0;
     const int st = sm_count(&sms);
     if (st != ESMM_OK) return st;
     if (out8) {
-        if (dtype == ESMM_F32) return norm_launch_type<float, true, NORM>(p, vectors, sms, stream);
-        if (dtype == ESMM_F16) return norm_launch_type<__half, true, NORM>(p, vectors, sms, stream);
-        return norm_launch_type<__nv_bfloat16, true, NORM>(p, vectors, sms, stream);
+        if (dtype == ESMM_F32) return norm_launch_type<float, true, NORM>(p, aligned, sms, stream);
+        if (dtype == ESMM_F16) return norm_launch_type<__half, true, NORM>(p, aligned, sms, stream);
+        return norm_launch_type<__nv_bfloat16, true, NORM>(p, aligned, sms, stream);
     }
     if constexpr (NORM) {
-        if (dtype == ESMM_F32) return norm_launch_type<float, false, true>(p, vectors, sms, stream);
-        if (dtype == ESMM_F16) return norm_launch_type<__half, false, true>(p, vectors, sms, stream);
-        return norm_launch_type<__nv_bfloat16, false, true>(p, vectors, sms, stream);
+        if (dtype == ESMM_F32) return norm_launch_type<float, false, true>(p, aligned, sms, stream);
+        if (dtype == ESMM_F16) return norm_launch_type<__half, false, true>(p, aligned, sms, stream);
+        return norm_launch_type<__nv_bfloat16, false, true>(p, aligned, sms, stream);
     }
     return ESMM_ERR_UNSUPPORTED;
 }
+
+template <int N> struct Num { static constexpr int value = N; };
 
 static bool row_dtype(int dtype) { return dtype == ESMM_F32 || dtype == ESMM_F16 || dtype == ESMM_BF16; }
 
 static bool element_aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
+constexpr int RING_BYTES = 200 * 1024;   // of a backward pass's rows under way, per SM
+
+// Raises a kernel's shared-memory allowance to the device's maximum, once per device.
+template <auto KERNEL>
+static int allow_ring()
+{
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    ESMM_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+        ESMM_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES + 1024));
+        if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+    }
+    return ESMM_OK;
+}
+
 template <typename T>
-static int norm_backward_type(const NormGradParams &p, bool vectors, int sms, int *ctas, cudaStream_t stream)
+static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas, cudaStream_t stream)
 {
     constexpr int VEC = 16 / (int)sizeof(T);
-    auto go = [&](auto kernel, int threads) -> int {
-        int per_sm = 0;
-        ESMM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0));
-        *ctas = std::max(1, std::min(std::min(p.M, ROWS_MAX_PARTIALS), sms * std::max(1, std::min(per_sm, 4))));
-        ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads), 0, stream, p));
+    const bool vectors = aligned && p.K % VEC == 0;
+    p.row_bytes = ceil_div(p.K * (int)sizeof(T), 16) * 16 + (vectors ? 0 : 16);
+    auto go = [&](auto tag, auto nv, auto most, auto keep) -> int {
+        constexpr int V = decltype(tag)::value, N = decltype(nv)::value;
+        constexpr auto kernel = &esmm_rmsnorm_backward_kernel<T, V, N, decltype(most)::value, decltype(keep)::value != 0>;
+        const int threads = ceil_div(ceil_div(p.K, V * N), 32) * 32;
+        const int groups = threads == 32 ? std::min(4, p.M) : 1;
+        // As many rows under way as the SM's shared memory holds, two per group at least, in one to four CTAs per SM.  More CTAs leave
+        // more partial rows of dw to add up; they pay for short rows where each has many (one / two / four CTAs per SM, us: 8192 x 4096
+        // bf16 67 / 46 / 52, 8192 x 1021 bf16 104 / 60 / 40, 1003 x 1509 fp32 16.9 / 12.7 / 15.3, 4096 x 4096 fp32 45 / 48.5 / 48.5).
+        int per_sm = threads > 256 ? 1 : threads <= 128 && groups == 1 && p.M >= 32 * sms ? 4 : 2;
+        while (per_sm > 1 && RING_BYTES / per_sm < 2 * groups * 3 * p.row_bytes) --per_sm;
+        *ctas = std::max(1, std::min(std::min(ceil_div(p.M, groups), ROWS_MAX_PARTIALS), sms * per_sm));
+        p.stages = std::max(1, std::min({8, RING_BYTES / per_sm / (groups * 3 * p.row_bytes), ceil_div(p.M, *ctas * groups)}));
+        // (the groups' sums of dw are added up where the rings were)
+        const size_t smem = std::max((size_t)groups * p.stages * (3 * p.row_bytes + 8), groups > 1 ? (size_t)groups * threads * N * V * 4 : 0);
+        const int st = allow_ring<kernel>();
+        if (st != ESMM_OK) return st;
+        ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads, groups), smem, stream, p));
         return ESMM_OK;
     };
-    auto threads_for = [&](int vec, int nv) { return ceil_div(ceil_div(p.K, vec * nv), 32) * 32; };
-    if (vectors) {
-        const int units = ceil_div(p.K, VEC);
-        if (units <= 512) return go(esmm_rmsnorm_backward_kernel<T, VEC, 1>, threads_for(VEC, 1));
-        if (units <= 2048) return go(esmm_rmsnorm_backward_kernel<T, VEC, 2>, threads_for(VEC, 2));
-    } else {
-        if (p.K <= 2048) return go(esmm_rmsnorm_backward_kernel<T, 1, 4>, threads_for(1, 4));
-        if (p.K <= 8192) return go(esmm_rmsnorm_backward_kernel<T, 1, 8>, threads_for(1, 8));
+    if (aligned && 2 * 3 * p.row_bytes <= RING_BYTES) {
+        if (vectors && p.K <= 32 * VEC) return go(Num<VEC>(), Num<1>(), Num<128>(), Num<1>());
+        if (vectors && p.K <= 64 * VEC) return go(Num<VEC>(), Num<2>(), Num<128>(), Num<1>());
+        if (vectors && VEC == 8 && p.K <= 128 * VEC) return go(Num<VEC>(), Num<4>(), Num<128>(), Num<1>());
+        if (vectors && p.K <= 512 * VEC) return go(Num<VEC>(), Num<2>(), Num<256>(), Num<1>());
+        if (vectors && p.K <= 1024 * VEC) return go(Num<VEC>(), Num<2>(), Num<512>(), Num<1>());
+        if (vectors && p.K <= 2048 * VEC) return go(Num<VEC>(), Num<4>(), Num<512>(), Num<0>());
+        if (!vectors && p.K <= 128) return go(Num<1>(), Num<4>(), Num<128>(), Num<1>());
+        if (!vectors && p.K <= 4096) return go(Num<1>(), Num<8>(), Num<512>(), Num<1>());
+        if (!vectors && p.K <= 8192) return go(Num<1>(), Num<8>(), Num<1024>(), Num<0>());
     }
-    return go(esmm_rmsnorm_backward_long_kernel<T>, 1024);
+    *ctas = std::max(1, std::min(std::min(p.M, ROWS_MAX_PARTIALS), 2 * sms));
+    ESMM_CUDA_TRY(launch_dependent(esmm_rmsnorm_backward_long_kernel<T>, dim3((unsigned)*ctas), dim3(1024), 0, stream, p));
+    return ESMM_OK;
 }
 
 static int column_sum(const float *partial, int rows, int K, int dtype, void *out, cudaStream_t stream)
 {
     auto go = [&](auto tag) -> int {
         typedef decltype(tag) T;
-        ESMM_CUDA_TRY(launch_dependent(esmm_column_sum_kernel<T>, dim3((unsigned)ceil_div(K, 32)), dim3(32, 32), 0, stream, partial, rows, K,
+        ESMM_CUDA_TRY(launch_dependent(esmm_column_sum_kernel<T>, dim3((unsigned)ceil_div(K, 32)), dim3(8, 64), 0, stream, partial, rows, K,
                                        static_cast<T *>(out)));
         return ESMM_OK;
     };
@@ -661,8 +976,7 @@ int esmm_rmsnorm(int M, int K, int dtype, const void *d_x, const void *d_residua
     p.rstd = d_rstd;
     p.status = device_status_ptr();
     if (!p.status) return ESMM_ERR_CUDA;
-    const bool vectors = K % (16 / size) == 0 && aligned16({d_x, d_residual, d_weight, d_sum, d_out});
-    return norm_launch<true>(p, dtype, out8, vectors, (cudaStream_t)stream);
+    return norm_launch<true>(p, dtype, out8, aligned16({d_x, d_residual, d_weight, d_sum, d_out}), (cudaStream_t)stream);
 }
 
 int esmm_quantize_rows(int M, int K, int dtype, const void *d_x, void *d_out, float *d_scale, void *stream)
@@ -682,7 +996,7 @@ int esmm_quantize_rows(int M, int K, int dtype, const void *d_x, void *d_out, fl
     p.scale = d_scale;
     p.status = device_status_ptr();
     if (!p.status) return ESMM_ERR_CUDA;
-    return norm_launch<false>(p, dtype, true, K % (16 / size) == 0 && aligned16({d_x, d_out}), (cudaStream_t)stream);
+    return norm_launch<false>(p, dtype, true, aligned16({d_x, d_out}), (cudaStream_t)stream);
 }
 
 size_t esmm_rmsnorm_backward_workspace_bytes(int M, int K)
@@ -719,10 +1033,10 @@ int esmm_rmsnorm_backward(int M, int K, int dtype, const void *d_dout, const voi
     int sms = 0, ctas = 0;
     int st = sm_count(&sms);
     if (st != ESMM_OK) return st;
-    const bool vectors = K % (16 / size) == 0 && aligned16({d_dout, d_h, d_weight, d_dsum, d_dx});
-    if (dtype == ESMM_F32) st = norm_backward_type<float>(p, vectors, sms, &ctas, stream);
-    else if (dtype == ESMM_F16) st = norm_backward_type<__half>(p, vectors, sms, &ctas, stream);
-    else st = norm_backward_type<__nv_bfloat16>(p, vectors, sms, &ctas, stream);
+    const bool aligned = aligned16({d_dout, d_h, d_weight, d_dsum, d_dx});
+    if (dtype == ESMM_F32) st = norm_backward_type<float>(p, aligned, sms, &ctas, stream);
+    else if (dtype == ESMM_F16) st = norm_backward_type<__half>(p, aligned, sms, &ctas, stream);
+    else st = norm_backward_type<__nv_bfloat16>(p, aligned, sms, &ctas, stream);
     if (st != ESMM_OK || !d_dweight) return st;
     return column_sum(p.partial, ctas, K, dtype, d_dweight, stream);
 }

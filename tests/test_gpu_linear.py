@@ -60,7 +60,7 @@ def test_sizes(cuda, pkg, t, m, n, k):
     check(pkg, m, n, k, t, out="f16" if t == "e4m3" else t, activation="silu", bias=True, residual=True, pre=True, scales=True, seed=3)
 
 
-@pytest.mark.parametrize("pair", [0, 128, 256])
+@pytest.mark.parametrize("pair", [0, 64, 128, 192, 256])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (40, 72, 72), (256, 256, 64), (264, 520, 200), (1000, 1512, 328)])
 @pytest.mark.parametrize("trans", ["nn", "nt", "tn"])
 def test_kernels_and_layouts(cuda, pkg, tuning, pair, m, n, k, trans):
@@ -71,7 +71,7 @@ def test_kernels_and_layouts(cuda, pkg, tuning, pair, m, n, k, trans):
         check(pkg, m, n, k, t, trans_a=trans == "tn", trans_b=trans == "nt", activation="gelu", bias=True, residual=True, pre=True)
 
 
-@pytest.mark.parametrize("pair", [0, 128, 256])
+@pytest.mark.parametrize("pair", [0, 64, 128, 192, 256])
 def test_e4m3_kernels(cuda, pkg, tuning, pair):
     tuning("LINEAR_PAIR", pair)
     for (m, n, k) in [(1, 8, 16), (264, 520, 400), (700, 776, 1168)]:
@@ -97,7 +97,7 @@ def test_epilogue_parts(cuda, pkg, tuning, activation, pair):
               seed=bits)
 
 
-@pytest.mark.parametrize("pair", [0, 128, 256])
+@pytest.mark.parametrize("pair", [0, 64, 128, 192, 256])
 def test_residual_in_place(cuda, pkg, tuning, pair):
     tuning("LINEAR_PAIR", pair)
     check(pkg, 300, 328, 128, "f16", bias=True, residual=True, inplace=True, activation="relu")
