@@ -50,7 +50,7 @@ int record_cuda_error(cudaError_t e, const char *what)
 // ---------------------------------------------------------------------------
 static const char *const kTuningNames[] = {"TILE_M", "STAGES", "BROW_BITS", "ROW_DENSITY", "FORCE_LISTED", "NO_RUN_TILES",
                                            "VEC_PATTERNS", "NO_SKINNY", "SKINNY_ROWS", "PRODUCER_WARPS", "BLOCK_MODE", "NO_DEPENDENT_LAUNCH", "GROUP_M", "GRID", "PACK", "SWIZZLE", "TF32_PAIR",
-                                           "TF32_SPLIT_LAST", "TF32_DIRECT_STORES", "LINEAR_PAIR", "LINEAR_SPLIT", "LINEAR_COLUMNS"};
+                                           "TF32_SPLIT_LAST", "TF32_DIRECT_STORES", "LINEAR_PAIR", "LINEAR_TAIL", "LINEAR_SPLIT", "LINEAR_COLUMNS"};
 constexpr int kTuningCount = (int)(sizeof kTuningNames / sizeof kTuningNames[0]);
 static std::atomic<int> g_tuning_value[kTuningCount];
 static std::atomic<bool> g_tuning_set[kTuningCount];

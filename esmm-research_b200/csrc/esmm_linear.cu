@@ -26,22 +26,30 @@
 
 namespace esmm {
 
+// What depends on a tile's width
+struct LinearTile {
+    int nb, tiles_n;                     // columns of a tile, tiles across
+    int b_boxes, b_box_cols, b_box_bytes;   // copies of B per stage (K-major: one), columns and bytes of one
+    int stage_bytes;                     // pair kernel: bytes that a CTA copies per stage
+    uint32_t b_desc_hi, b_lbo, b_step;   // B's descriptors: high word, leading byte offset in place, from one MMA to the next
+    uint32_t idesc;
+};
+
 struct LinearParams {
     int M, N, ksteps;                    // K in steps of 128 bytes
-    int tiles_m, tiles_n, num_tiles;
+    int tiles_m, num_tiles;
+    // pair kernel: the first `wide_tiles` tiles cover the columns before `wide_cols` in the first width, the rest the others in the second
+    LinearTile kind[2];
+    int wide_tiles, wide_cols;
     int group_m;
-    int a_boxes, b_boxes;                // copies per stage and operand
+    int a_boxes;                         // copies of A per stage
     int a_k_major, b_k_major;
     int k_elems;                         // elements of K per step
     int stages;
     int a_stage_bytes;                   // split kernel: of A's part of a stage
-    uint32_t idesc;
-    uint32_t a_lbo, b_lbo;               // leading byte offset of the descriptors, in place
-    uint32_t b_desc_hi;                  // the high word of B's descriptors
-    int b_box_bytes, b_box_cols;         // MN-major B: one of its boxes
-    int nb;                              // pair kernel: columns of a tile
-    int stage_bytes;                     // pair kernel
-    uint32_t a_step, b_step;             // from one MMA to the next along K, in 16-byte units
+    int slot_bytes;                      // pair kernel: from one ring slot to the next
+    uint32_t a_lbo;                      // leading byte offset of A's descriptors, in place
+    uint32_t a_step;                     // from one MMA to the next along K, in 16-byte units
     int bf16;                            // type of C, bias, residual and pre: bfloat16 or float16
     int activation, has_pre, has_residual;
     const float *a_scale, *b_scale;
@@ -52,7 +60,7 @@ struct LinearParams {
 };
 
 struct LinearMaps {
-    CUtensorMap a, b;
+    CUtensorMap a, b[2];                 // (b by the tiles' width)
     CUtensorMap c, residual, pre;        // pair kernel: boxes of 64 columns x 32 rows, 128-byte swizzle
 };
 
@@ -91,12 +99,12 @@ __device__ __forceinline__ bool linear_elect()
 // uniform registers, where the instruction wants them: from a lane's own branch every MMA took 68 cycles to issue, more
 // than an MMA of 64 columns runs.
 template <bool PAIR, bool F8>
-__device__ __forceinline__ void linear_mma_step(const LinearParams &p, uint32_t d, uint32_t a, uint32_t b, bool more, bool elected)
+__device__ __forceinline__ void linear_mma_step(const LinearParams &p, const LinearTile &t, uint32_t d, uint32_t a, uint32_t b, bool more, bool elected)
 {
     if (elected) {
-        linear_mma<PAIR, F8>(d, a, b, p.b_desc_hi, p.idesc, more ? 1u : 0u);
+        linear_mma<PAIR, F8>(d, a, b, t.b_desc_hi, t.idesc, more ? 1u : 0u);
 #pragma unroll
-        for (uint32_t j = 1; j < 4; ++j) linear_mma<PAIR, F8>(d, a + j * p.a_step, b + j * p.b_step, p.b_desc_hi, p.idesc, 1u);
+        for (uint32_t j = 1; j < 4; ++j) linear_mma<PAIR, F8>(d, a + j * p.a_step, b + j * t.b_step, t.b_desc_hi, t.idesc, 1u);
     }
     __syncwarp();
 }
@@ -173,15 +181,15 @@ __device__ __forceinline__ void linear_prefetch(const CUtensorMap *map, int x, i
 // The copies of one K step: lanes 0 .. a_boxes - 1 fetch A, lanes 4 .. 4 + b_boxes - 1 fetch B.  row_a, row_b: first row of op(A) and
 // column of op(B) of this CTA's part of the tile.
 template <bool PAIR>
-__device__ __forceinline__ void linear_load_step(const LinearParams &p, const LinearMaps &maps, int lane, int step, int row_a, int row_b,
+__device__ __forceinline__ void linear_load_step(const LinearParams &p, const LinearTile &t, const LinearMaps &maps, const CUtensorMap *b_map, int lane, int step, int row_a, int row_b,
                                                  uint32_t dst_a, uint32_t dst_b, uint32_t bar)
 {
     const bool is_b = lane >= 4;
     const int i = lane & 3;
-    if (lane >= 8 || i >= (is_b ? p.b_boxes : p.a_boxes)) return;
-    const int k = step * p.k_elems, r = is_b ? row_b + p.b_box_cols * i : row_a + 64 * i;
+    if (lane >= 8 || i >= (is_b ? t.b_boxes : p.a_boxes)) return;
+    const int k = step * p.k_elems, r = is_b ? row_b + t.b_box_cols * i : row_a + 64 * i;
     const bool k_major = is_b ? p.b_k_major : p.a_k_major;
-    linear_load<PAIR>(is_b ? dst_b + (uint32_t)(p.b_box_bytes * i) : dst_a + 8192u * (uint32_t)i, is_b ? &maps.b : &maps.a, k_major ? k : r, k_major ? r : k, bar);
+    linear_load<PAIR>(is_b ? dst_b + (uint32_t)(t.b_box_bytes * i) : dst_a + 8192u * (uint32_t)i, is_b ? b_map : &maps.a, k_major ? k : r, k_major ? r : k, bar);
 }
 
 // z: 32 sums of one row, columns c0 .. c0 + 31; scale and bias by column in shared memory.
@@ -207,6 +215,17 @@ constexpr int LP_BAR_OFF = LP_COLUMN_OFF + LP_EPI_WARPS * 256;
 constexpr int LP_SMEM = LP_BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
 constexpr int LP_TMEM_COLS = 2 * LP_MAX_NB;
 static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
+
+// Tile `item` of the launch: its width, tile row and first column.
+__device__ __forceinline__ const LinearTile &linear_tile(const LinearParams &p, int item, int &second, int &tm, int &col)
+{
+    second = item >= p.wide_tiles;
+    const LinearTile &t = p.kind[second];
+    int tn;
+    tile_coords(second ? item - p.wide_tiles : item, p.tiles_m, t.tiles_n, tm, tn, p.group_m);
+    col = (second ? p.wide_cols : 0) + tn * t.nb;
+    return t;
+}
 
 template <bool F8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LP_THREADS, 1)
@@ -254,22 +273,22 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     if (warp < L_PRODUCERS) {
         // ---------------- producers: K steps in turn ----------------
         if (lane == 0) tma_prefetch_descriptor(&maps.a);
-        if (lane == 4) tma_prefetch_descriptor(&maps.b);
+        if (lane == 4) tma_prefetch_descriptor(&maps.b[0]);
         int slot = warp, first = warp;                     // the slot of this warp's next step, and that step's index in the tile
         uint32_t phase = 0;
         for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
-            int tm, tn;
-            tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
-            const int row_a = tm * 256 + (int)rank * 128, row_b = tn * p.nb + (int)rank * (p.nb / 2);
+            int second, tm, col;
+            const LinearTile &t = linear_tile(p, tile, second, tm, col);
+            const int row_a = tm * 256 + (int)rank * 128, row_b = col + (int)rank * (t.nb / 2);
             int step = first;
             for (; step < p.ksteps; step += L_PRODUCERS) {
                 ok = mbar_wait(empty0 + 8 * slot, phase ^ 1, abort_flag);
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
-                if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * (uint32_t)p.stage_bytes);
+                if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * (uint32_t)t.stage_bytes);
                 __syncwarp();
-                const uint32_t dst = smem_u32(smem) + (uint32_t)(slot * p.stage_bytes);
-                linear_load_step<true>(p, maps, lane, step, row_a, row_b, dst, dst + LP_A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
+                const uint32_t dst = smem_u32(smem) + (uint32_t)(slot * p.slot_bytes);
+                linear_load_step<true>(p, t, maps, &maps.b[second], lane, step, row_a, row_b, dst, dst + LP_A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
                 slot += L_PRODUCERS;
                 if (slot >= p.stages) {
                     slot -= p.stages;
@@ -292,16 +311,17 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 linear_fence_after();
+                const LinearTile &t = p.kind[tile >= p.wide_tiles];
                 const uint32_t d = tmem + ab * (uint32_t)LP_MAX_NB;
                 for (int step = 0; step < p.ksteps; ++step) {
                     if (!landed) ok = mbar_wait(full0 + 8 * slot, phase, abort_flag);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
-                    const uint32_t at = ring + (uint32_t)(slot * (p.stage_bytes >> 4));
+                    const uint32_t at = ring + (uint32_t)(slot * (p.slot_bytes >> 4));
                     const int nslot = slot + 1 == p.stages ? 0 : slot + 1;
                     // (a wait costs time even where the data is there: ask for the next step's while this one's MMAs are issued)
                     landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
-                    linear_mma_step<true, F8>(p, d, at | p.a_lbo, (at + (LP_A_BYTES >> 4)) | p.b_lbo, step != 0, elected);
+                    linear_mma_step<true, F8>(p, t, d, at | p.a_lbo, (at + (LP_A_BYTES >> 4)) | t.b_lbo, step != 0, elected);
                     if (elected) linear_commit<true>(empty0 + 8 * slot);
                     landed = __all_sync(0xFFFFFFFFu, landed);
                     if (++slot == p.stages) {
@@ -317,16 +337,16 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     } else if (warp >= 4) {
         // ---------------- epilogue: a row per thread, 64 columns at a time through the warp's staging boxes ----------------
         const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns 64 (half + 2 c) ..
-        const int chunks = (p.nb / 64 - half + 1) / 2;            // of the tile's 64-column pieces, every other one: none to two
         constexpr int CHUNKS = 2;
         char *box = smem + LP_RING + w * LP_STAGING;
         float *col_scale = reinterpret_cast<float *>(smem + LP_COLUMN_OFF + w * 256), *col_bias = col_scale + 32;
         const uint32_t res_bar = res0 + 8 * w;
         uint32_t turn = 0, res_phase = 0;
         for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs, ++turn) {
-            int tm, tn;
-            tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
-            const int row0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tn * p.nb + half * 64;
+            int second, tm, col0;
+            const int chunks = (linear_tile(p, tile, second, tm, col0).nb / 64 - half + 1) / 2;   // of the tile's 64-column pieces, every other one: none to two
+            const int row0 = tm * 256 + (int)rank * 128 + q * 32;
+            col0 += half * 64;
             const uint32_t ab = turn & 1u;
             const bool residual_here = p.has_residual && chunks > 0 && row0 < p.M && col0 < p.N;
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the boxes are free again
@@ -547,7 +567,8 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
     const int rank = (int)linear_cta_rank();
     const int tile = blockIdx.x / split;
     int tm, tn;
-    tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn, p.group_m);
+    const LinearTile &t = p.kind[0];
+    tile_coords(tile, p.tiles_m, t.tiles_n, tm, tn, p.group_m);
     const int s0 = (int)((long)p.ksteps * rank / split), s1 = (int)((long)p.ksteps * (rank + 1) / split);   // this CTA's K steps, one at least
     const int row0 = tm * 128, col0 = tn * NB, rows = min(128, p.M - row0);
     constexpr int B_BYTES = NB * L_KBYTES;
@@ -573,10 +594,10 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
     grid_launch_dependents();
     // The first K steps of B are brought into L2 while the kernel before this one finishes (only there: should that kernel write B, what is
     // read after the wait is what it wrote).
-    if (warp >= LS_DRAIN_WARPS && warp < LS_DRAIN_WARPS + L_PRODUCERS && lane < p.b_boxes) {
+    if (warp >= LS_DRAIN_WARPS && warp < LS_DRAIN_WARPS + L_PRODUCERS && lane < t.b_boxes) {
         for (int i = warp - LS_DRAIN_WARPS; i < p.stages && s0 + i < s1; i += L_PRODUCERS) {
-            const int k = (s0 + i) * p.k_elems, r = col0 + p.b_box_cols * lane;
-            linear_prefetch(&maps.b, p.b_k_major ? k : r, p.b_k_major ? r : k);
+            const int k = (s0 + i) * p.k_elems, r = col0 + t.b_box_cols * lane;
+            linear_prefetch(&maps.b[0], p.b_k_major ? k : r, p.b_k_major ? r : k);
         }
     }
     grid_dependency_wait();
@@ -593,7 +614,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, (uint32_t)(p.a_stage_bytes + B_BYTES));
             __syncwarp();
-            linear_load_step<false>(p, maps, lane, step, row0, col0, a_ring + (uint32_t)(slot * p.a_stage_bytes), b_ring + (uint32_t)(slot * B_BYTES),
+            linear_load_step<false>(p, t, maps, &maps.b[0], lane, step, row0, col0, a_ring + (uint32_t)(slot * p.a_stage_bytes), b_ring + (uint32_t)(slot * B_BYTES),
                                     full0 + 8 * slot);
             slot += L_PRODUCERS;
             if (slot >= p.stages) {
@@ -613,8 +634,8 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             if (!ok) break;
             const int nslot = slot + 1 == p.stages ? 0 : slot + 1;
             landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
-            linear_mma_step<false, F8>(p, tmem, (a0 + (uint32_t)(slot * (p.a_stage_bytes >> 4))) | p.a_lbo,
-                                       (b0 + (uint32_t)(slot * (B_BYTES >> 4))) | p.b_lbo, step > s0, elected);
+            linear_mma_step<false, F8>(p, t, tmem, (a0 + (uint32_t)(slot * (p.a_stage_bytes >> 4))) | p.a_lbo,
+                                       (b0 + (uint32_t)(slot * (B_BYTES >> 4))) | t.b_lbo, step > s0, elected);
             if (elected) linear_commit<false>(empty0 + 8 * slot);
             landed = __all_sync(0xFFFFFFFFu, landed);
             if (++slot == p.stages) {
@@ -721,24 +742,37 @@ static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner,
 
 struct LinearChoice {
     int pair_nb;          // 64, 128, 192, 256: the width of the pair kernel's tiles; 0: the split kernel
+    int tail_nb, columns; // pair kernel: from this tile column on, tiles of another width
     int nb, split;        // split kernel
 };
 
-// Which kernel, tile width and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
+// Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
 // shapes (M = 1 .. 2048; K and N from 512 to 11008; 16 and 8 bits, B 0.25 to 90 MB, three sets of operands in turn): what the rule picks takes
-// 1.6 % longer than the best variant on average, 13 % at most.
+// 1.5 % longer than the best variant on average, 18 % at most.
 static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
 {
-    LinearChoice c = {0, 128, 1};
-    const int pairs = std::max(1, sms / 2);
+    LinearChoice c = {0, 0, 0, 128, 1};
+    const int pairs = std::max(1, sms / 2), down = ceil_div(M, 256);
     const double hbm = ((double)M + N) * ksteps * L_KBYTES / 6.5e6;            // operands once
     double best = 1e30;
+    // a K step: the MMAs, or the copies, which are slower the more SMs copy
+    auto step = [&](int nb, long tiles) {
+        return std::max(nb * 0.00127, (256 + nb) * (0.000256 + 0.0003 * (double)std::min<long>(tiles, pairs) / pairs));
+    };
     for (int nb = 64; nb <= 256; nb += 64) {
-        const long tiles = (long)ceil_div(M, 256) * ceil_div(N, nb), rounds = (tiles + pairs - 1) / pairs;
-        // a K step: the MMAs, or the copies, which are slower the more SMs copy
-        const double step = std::max(nb * 0.00152, (256 + nb) * (0.000337 + 0.000268 * (double)std::min<long>(tiles, pairs) / pairs));
-        const double t = 4.07 + 0.11 * nb / 64 + std::max(rounds * ksteps * step, hbm) + 1.4 * (rounds - 1);
-        if (t < best) best = t, c.pair_nb = nb;
+        const int across = ceil_div(N, nb);
+        const long tiles = (long)down * across, rounds = (tiles + pairs - 1) / pairs;
+        const double fixed = 3.9 + 0.68 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm);
+        if (t < best) best = t, c.pair_nb = nb, c.columns = c.tail_nb = 0;
+        // where the last round is partly filled: whole rounds of this width, the columns that are left in narrower tiles
+        const int columns = (int)std::min<long>(across, tiles / pairs * pairs / down);
+        if (columns < 1 || columns == across) continue;
+        for (int tail = 64; tail < nb; tail += 64) {
+            const long first = (long)columns * down, all = first + (long)ceil_div(N - columns * nb, tail) * down;
+            const long wide = (first + pairs - 1) / pairs, narrow = (all + pairs - 1) / pairs - wide;
+            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm);
+            if (tt < 0.98 * best) best = tt, c.pair_nb = nb, c.tail_nb = tail, c.columns = columns;
+        }
     }
     const int rows = std::min(M, 128), box = ceil_div(rows, 8) * 8;
     for (int nb = 64; nb <= 128; nb += 64) {
@@ -748,14 +782,19 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
             const long ctas = tiles * split, rounds = (ctas + 2 * sms - 1) / (2 * sms);
             const int steps = ceil_div(ksteps, split);
             const double kb = (box + nb) * (L_KBYTES / 1000.0);                // copied per step and CTA
-            const double one = rounds * steps * std::max(0.253, kb / 75.0), all = ctas * steps * kb / 17450.0;
-            const double t = 3.55 + 0.31 * rows * nb / 16384 + std::max({one, all, hbm}) + 1.6 * (rounds - 1) +
-                             (split - 1) * (0.19 + (double)M * N * 4 / 1.9e6);  // sums through distributed shared memory
-            if (t < best) best = t, c = {0, nb, split};
+            const double one = rounds * steps * std::max(0.179, kb / 82.6), all = ctas * steps * kb / 17700.0;
+            // (fewer CTAs than the SMs have room for have less of HBM under way)
+            const double bytes = hbm * (1.0 + 0.5 * (1.0 - (double)ctas / (rounds * 2 * sms)));
+            const double t = 3.2 + 2.6 * rows * nb / 16384 + std::max({one, all, bytes}) + 1.8 * (rounds - 1) +
+                             (split - 1) * (0.077 + (double)M * N * 4 / 3.46e6);   // sums through distributed shared memory
+            if (t < best) best = t, c = {0, 0, 0, nb, split};
         }
     }
     const int forced = tuning_get("LINEAR_PAIR", -1);
-    if (forced == 0 || forced == 64 || forced == 128 || forced == 192 || forced == 256) c.pair_nb = forced;
+    if (forced == 0 || forced == 64 || forced == 128 || forced == 192 || forced == 256) c.pair_nb = forced, c.columns = c.tail_nb = 0;
+    const int forced_tail = tuning_get("LINEAR_TAIL", 0);
+    if (c.pair_nb && forced_tail > 0 && forced_tail < c.pair_nb && forced_tail % 64 == 0 && N > c.pair_nb)
+        c.tail_nb = forced_tail, c.columns = (ceil_div(N, c.pair_nb) + 1) / 2;
     const int forced_split = tuning_get("LINEAR_SPLIT", 0);
     if (forced_split >= 1 && forced_split <= LS_MAX_SPLIT) c.split = std::min(forced_split, ksteps);
     const int forced_nb = tuning_get("LINEAR_COLUMNS", 0);
@@ -817,30 +856,35 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
 
     const LinearChoice choice = linear_choose(M, N, p.ksteps, sms);
     const int rows_a = 128;                                                 // rows of A per CTA
-    const int cols_b = choice.pair_nb ? choice.pair_nb / 2 : choice.nb;     // columns of B per CTA
     // few rows: boxes of as many as there are (what the MMA reads past them is never looked at)
     int a_box_rows = rows_a;
     if (!choice.pair_nb && p.a_k_major && M < rows_a) a_box_rows = ceil_div(M, 8) * 8;
     p.a_boxes = p.a_k_major ? 1 : rows_a / 64;
-    // MN-major B in boxes of 64 columns, or of 32 with the 64-byte swizzle where a CTA's columns are no multiple of 64
-    const bool wide = cols_b % 64 == 0;
-    p.b_box_cols = p.b_k_major ? cols_b : wide ? 64 : 32;
-    p.b_box_bytes = p.b_box_cols * (p.b_k_major ? L_KBYTES : 128);
-    p.b_boxes = cols_b / p.b_box_cols;
-    p.b_desc_hi = p.b_k_major || wide ? L_DESC_HI : L_DESC_HI_64;
-    p.b_step = p.b_k_major ? 2u : wide ? 128u : 64u;
-    p.b_lbo = (p.b_k_major ? 1u : (uint32_t)p.b_box_bytes >> 4) << 16;
-    // D = F32; A and B: F16 0, BF16 1, E4M3 0; bits 15, 16: MN-major; N >> 3, M >> 4
-    const uint32_t ab_type = dtype == ESMM_BF16 ? 1u : 0u;
-    const uint32_t mma_m = choice.pair_nb ? 256u : 128u, mma_n = (uint32_t)(choice.pair_nb ? choice.pair_nb : choice.nb);
-    p.idesc = (1u << 4) | (ab_type << 7) | (ab_type << 10) | ((p.a_k_major ? 0u : 1u) << 15) | ((p.b_k_major ? 0u : 1u) << 16) |
-              ((mma_n >> 3) << 17) | ((mma_m >> 4) << 24);
-
     LinearMaps maps;
     memset(&maps, 0, sizeof maps);
     st = p.a_k_major ? linear_map(&maps.a, dtype, d_A, K, M, p.k_elems, a_box_rows) : linear_map(&maps.a, dtype, d_A, M, K, 64, 64);
-    if (!st) st = p.b_k_major ? linear_map(&maps.b, dtype, d_B, K, N, p.k_elems, cols_b) : linear_map(&maps.b, dtype, d_B, N, K, p.b_box_cols, 64, wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (st) return st;
+    for (int i = 0; i < (choice.tail_nb ? 2 : 1); ++i) {
+        LinearTile &t = p.kind[i];
+        t.nb = i ? choice.tail_nb : choice.pair_nb ? choice.pair_nb : choice.nb;
+        const int cols = choice.pair_nb ? t.nb / 2 : t.nb;                  // columns of B per CTA
+        // MN-major B in boxes of 64 columns, or of 32 with the 64-byte swizzle where a CTA's columns are no multiple of 64
+        const bool wide = cols % 64 == 0;
+        t.b_box_cols = p.b_k_major ? cols : wide ? 64 : 32;
+        t.b_box_bytes = t.b_box_cols * 128;                                 // 128 bytes of K, or 64 k of two bytes each, per column
+        t.b_boxes = cols / t.b_box_cols;
+        t.stage_bytes = LP_A_BYTES + cols * L_KBYTES;
+        t.b_desc_hi = p.b_k_major || wide ? L_DESC_HI : L_DESC_HI_64;
+        t.b_step = p.b_k_major ? 2u : wide ? 128u : 64u;
+        t.b_lbo = (p.b_k_major ? 1u : (uint32_t)t.b_box_bytes >> 4) << 16;
+        // D = F32; A and B: F16 0, BF16 1, E4M3 0; bits 15, 16: MN-major; N >> 3, M >> 4
+        const uint32_t ab_type = dtype == ESMM_BF16 ? 1u : 0u, mma_m = choice.pair_nb ? 256u : 128u;
+        t.idesc = (1u << 4) | (ab_type << 7) | (ab_type << 10) | ((p.a_k_major ? 0u : 1u) << 15) | ((p.b_k_major ? 0u : 1u) << 16) |
+                  (((uint32_t)t.nb >> 3) << 17) | ((mma_m >> 4) << 24);
+        st = p.b_k_major ? linear_map(&maps.b[i], dtype, d_B, K, N, p.k_elems, cols)
+                         : linear_map(&maps.b[i], dtype, d_B, N, K, t.b_box_cols, 64, wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+        if (st) return st;
+    }
 
     if (choice.pair_nb) {
         st = linear_map(&maps.c, out_dtype, d_C, N, M, 64, 32);
@@ -848,13 +892,15 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
         if (!st && d_pre) st = linear_map(&maps.pre, out_dtype, d_pre, N, M, 64, 32);
         if (st) return st;
         p.tiles_m = ceil_div(M, 256);
-        p.tiles_n = ceil_div(N, choice.pair_nb);
-        if ((long)p.tiles_m * p.tiles_n > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
-        p.num_tiles = p.tiles_m * p.tiles_n;
+        p.kind[0].tiles_n = choice.tail_nb ? choice.columns : ceil_div(N, choice.pair_nb);
+        p.wide_cols = p.kind[0].tiles_n * choice.pair_nb;
+        if (choice.tail_nb) p.kind[1].tiles_n = ceil_div(N - p.wide_cols, choice.tail_nb);
+        if ((long)p.tiles_m * (p.kind[0].tiles_n + p.kind[1].tiles_n) > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
+        p.wide_tiles = p.tiles_m * p.kind[0].tiles_n;
+        p.num_tiles = p.wide_tiles + p.tiles_m * p.kind[1].tiles_n;
         const int pairs = std::max(1, std::min(sms / 2, p.num_tiles));
-        p.nb = choice.pair_nb;
-        p.stage_bytes = LP_A_BYTES + p.nb / 2 * L_KBYTES;
-        p.stages = std::min(LP_MAX_STAGES, LP_RING / p.stage_bytes);
+        p.slot_bytes = p.kind[0].stage_bytes;
+        p.stages = std::min(LP_MAX_STAGES, LP_RING / p.slot_bytes);
         auto go = [&](auto kernel) -> int {
             ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)LP_SMEM, stream, maps, p));
             return ESMM_OK;
@@ -863,9 +909,9 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     }
 
     p.tiles_m = ceil_div(M, 128);
-    p.tiles_n = ceil_div(N, choice.nb);
-    if ((long)p.tiles_m * p.tiles_n * choice.split > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
-    p.num_tiles = p.tiles_m * p.tiles_n;
+    p.kind[0].tiles_n = ceil_div(N, choice.nb);
+    if ((long)p.tiles_m * p.kind[0].tiles_n * choice.split > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
+    p.num_tiles = p.tiles_m * p.kind[0].tiles_n;
     p.a_stage_bytes = a_box_rows * L_KBYTES;
     const int b_stage = choice.nb * L_KBYTES, steps = ceil_div(p.ksteps, choice.split);
     // two CTAs per SM; the MMA reads 128 rows of A from any slot, so past the last one the B ring (16 KB at least) has to follow

@@ -419,20 +419,19 @@ struct NormGradParams {
     const float *rstd;
     void *dx;
     float *partial;      // one row of K sums per CTA
-    int stages, row_bytes;
+    int stages, row_bytes, bar_off;
     int *status;
 };
 
 // The rows come as bulk copies into a ring of `stages` rows of dout, h and dsum, some rows ahead: what is under way does not depend
-// on the registers of the threads that wait for a row's reduction.  A row that does not start on 16 bytes is copied from the boundary before
-// it to the one after it (VEC = 1: its elements are then read one by one); where the matrix ends in between, the last elements are read
-// from where they lie.  KEEP: a thread keeps its part of a row between the row's two passes, and the row's slot is free at once; for the
-// longest rows it reads the slot again.  8192 x 4096 of bf16, without dw: rows through registers, one ahead, 54.3 us; so 43.6 (HBM alone 41.0).
+// on the registers of the threads that wait for a row's reduction.  KEEP: a thread keeps its part of a row between the row's two passes,
+// and the row's slot is free at once; for the longest rows it reads the slot again.  us without dw, rows through registers one ahead / so /
+// HBM alone: 8192 x 4096 of bf16 54.3 / 42.5 / 41.0, 2048 x 11008 75 / 36 / 27.5.
 template <typename T, int VEC, int NV, int THREADS, bool KEEP>
 __global__ void __launch_bounds__(THREADS)
 esmm_rmsnorm_backward_kernel(const NormGradParams p)
 {
-    extern __shared__ __align__(16) char smem[];   // per group: [stage][dout, h, dsum][row_bytes]; then one barrier per group and stage
+    extern __shared__ __align__(16) char smem[];   // per group: [stage][dout, h, dsum][row_bytes]; from bar_off one barrier per group and stage
     __shared__ float slots[64];
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
@@ -440,9 +439,8 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
     // blockDim.y groups of blockDim.x threads have a row each (several only where a group is one warp)
     const int groups = blockDim.y, group = threadIdx.y;
     const char *ring = smem + (size_t)group * p.stages * 3 * p.row_bytes;
-    const uint32_t ring0 = smem_u32(ring), bars = smem_u32(smem) + (uint32_t)(groups * p.stages * 3 * p.row_bytes + group * p.stages * 8);
+    const uint32_t ring0 = smem_u32(ring), bars = smem_u32(smem) + (uint32_t)(p.bar_off + group * p.stages * 8);
     const T *weight = static_cast<const T *>(p.weight);
-    const size_t total = (size_t)p.M * p.K * sizeof(T);
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(bars + 8 * i, 1);
         abort_word = 0;
@@ -453,18 +451,14 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
     grid_launch_dependents();
     grid_dependency_wait();
     const bool adds = p.dsum != nullptr;
-    // bytes [lo, hi) of each array are copied for a row
-    auto row_lo = [&](size_t row) { return row * p.K * sizeof(T) & ~(size_t)15; };
-    auto row_hi = [&](size_t row) { return min(((row + 1) * p.K * sizeof(T) + 15) & ~(size_t)15, total & ~(size_t)15); };
+    const uint32_t bytes = (uint32_t)p.row_bytes;
     auto fetch = [&](size_t row, int slot) {
-        const size_t lo = row_lo(row);
-        const uint32_t bytes = (uint32_t)(row_hi(row) - lo), bar = bars + 8 * slot;
-        const uint32_t to = ring0 + (uint32_t)(slot * 3 * p.row_bytes);
+        const size_t from = row * bytes;
+        const uint32_t to = ring0 + (uint32_t)slot * 3u * bytes, bar = bars + 8 * slot;
         mbar_arrive_expect_tx(bar, bytes * (adds ? 3u : 2u));
-        if (!bytes) return;
-        bulk_load(to, static_cast<const char *>(p.dout) + lo, bytes, bar);
-        bulk_load(to + (uint32_t)p.row_bytes, static_cast<const char *>(p.h) + lo, bytes, bar);
-        if (adds) bulk_load(to + 2u * (uint32_t)p.row_bytes, static_cast<const char *>(p.dsum) + lo, bytes, bar);
+        bulk_load(to, static_cast<const char *>(p.dout) + from, bytes, bar);
+        bulk_load(to + bytes, static_cast<const char *>(p.h) + from, bytes, bar);
+        if (adds) bulk_load(to + 2u * bytes, static_cast<const char *>(p.dsum) + from, bytes, bar);
     };
     const size_t first = (size_t)blockIdx.x * groups + group, stride = (size_t)gridDim.x * groups;
     if (threadIdx.x == 0)
@@ -486,22 +480,9 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
     for (size_t row = first; row < (size_t)p.M; row += stride, turn ^= 32) {
         const size_t base = row * (size_t)p.K, next = row + stride;
         const float rstd_next = next < (size_t)p.M ? p.rstd[next] : 0.0f;
-        const char *g_at = ring + (size_t)slot * 3 * p.row_bytes + (VEC == 1 ? base * sizeof(T) - row_lo(row) : 0);
+        const char *g_at = ring + (size_t)slot * 3 * p.row_bytes;
         const char *h_at = g_at + p.row_bytes, *s_at = h_at + p.row_bytes;
-        // columns from this one on lie behind what was copied
-        const int copied = VEC == 1 ? (int)min((long long)p.K, ((long long)row_hi(row) - (long long)(base * sizeof(T))) / (long long)sizeof(T)) : p.K;
         ok = mbar_wait(bars + 8 * slot, phase, abort_flag) && ok;
-        if (VEC == 1 && copied < p.K) {               // the matrix's last elements, to where the copies would have put them
-            for (int c = max(copied, 0) + threadIdx.x; c < p.K; c += blockDim.x) {
-                const uint32_t o = (uint32_t)(slot * 3 * p.row_bytes) + (uint32_t)(base * sizeof(T) - row_lo(row));
-                T *to = reinterpret_cast<T *>(const_cast<char *>(ring) + o) + c;
-                to[0] = static_cast<const T *>(p.dout)[base + c];
-                *reinterpret_cast<T *>(reinterpret_cast<char *>(to) + p.row_bytes) = static_cast<const T *>(p.h)[base + c];
-                if (adds) *reinterpret_cast<T *>(reinterpret_cast<char *>(to) + 2 * p.row_bytes) = static_cast<const T *>(p.dsum)[base + c];
-            }
-            if (blockDim.x > 32) __syncthreads();
-            else __syncwarp();
-        }
         auto element = [&](const char *at, int c) { return *reinterpret_cast<const raw_t *>(at + (size_t)c * sizeof(T)); };
         raw_t s_raw[KEEP ? NV : 1];
         float gw[KEEP ? NV : 1][VEC], xh[KEEP ? NV : 1][VEC], dot[2] = {0.0f, 0.0f};
@@ -512,24 +493,17 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
             unpack<T, VEC>(element(g_at, c), gwi);
             unpack<T, VEC>(element(h_at, c), xhi);
             if (weight) unpack<T, VEC>(w[i], f);
-            if constexpr (VEC == 1) {
-                xhi[0] *= rstd;
-                if (sums) dw[i][0] = fmaf(gwi[0], xhi[0], dw[i][0]);
-                gwi[0] *= f[0];
-                if (sums) dot[0] = fmaf(gwi[0], xhi[0], dot[0]);
-            } else {                                // two at a time
 #pragma unroll
-                for (int j = 0; j < VEC; j += 2) {
-                    const float2 g2 = make_float2(gwi[j], gwi[j + 1]), x2 = __fmul2_rn(make_float2(xhi[j], xhi[j + 1]), make_float2(rstd, rstd));
-                    const float2 p2 = __fmul2_rn(g2, make_float2(f[j], f[j + 1]));
-                    if (sums) {
-                        const float2 d2 = __ffma2_rn(g2, x2, make_float2(dw[i][j], dw[i][j + 1])), s2 = __ffma2_rn(p2, x2, make_float2(dot[0], dot[1]));
-                        dw[i][j] = d2.x, dw[i][j + 1] = d2.y;
-                        dot[0] = s2.x, dot[1] = s2.y;
-                    }
-                    xhi[j] = x2.x, xhi[j + 1] = x2.y;
-                    gwi[j] = p2.x, gwi[j + 1] = p2.y;
+            for (int j = 0; j < VEC; j += 2) {
+                const float2 g2 = make_float2(gwi[j], gwi[j + 1]), x2 = __fmul2_rn(make_float2(xhi[j], xhi[j + 1]), make_float2(rstd, rstd));
+                const float2 p2 = __fmul2_rn(g2, make_float2(f[j], f[j + 1]));
+                if (sums) {
+                    const float2 d2 = __ffma2_rn(g2, x2, make_float2(dw[i][j], dw[i][j + 1])), s2 = __ffma2_rn(p2, x2, make_float2(dot[0], dot[1]));
+                    dw[i][j] = d2.x, dw[i][j + 1] = d2.y;
+                    dot[0] = s2.x, dot[1] = s2.y;
                 }
+                xhi[j] = x2.x, xhi[j + 1] = x2.y;
+                gwi[j] = p2.x, gwi[j + 1] = p2.y;
             }
         };
 #pragma unroll
@@ -542,6 +516,7 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
         }
         const float mean = row_reduce<false>(dot[0] + dot[1], slots + turn) / (float)p.K;
         // every thread has the row in its registers (or, !KEEP, is through with the row before it): that slot takes the next row
+        if (blockDim.x == 32) __syncwarp();
         if (threadIdx.x == 0) {
             const size_t ahead = row + (KEEP ? p.stages : p.stages - 1) * stride;
             if (ahead < (size_t)p.M && (KEEP || row != first)) fetch(ahead, KEEP ? slot : slot ? slot - 1 : p.stages - 1);
@@ -560,15 +535,11 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
                     if (adds) unpack<T, VEC>(element(s_at, c), add);
                     products(i, c, gw[0], xh[0], false);
                 }
-                if constexpr (VEC == 1) {
-                    gw[at][0] = fmaf(rstd, fmaf(-mean, xh[at][0], gw[at][0]), add[0]);
-                } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; j += 2) {
-                        const float2 g2 = __ffma2_rn(make_float2(-mean, -mean), make_float2(xh[at][j], xh[at][j + 1]), make_float2(gw[at][j], gw[at][j + 1]));
-                        const float2 o2 = __ffma2_rn(make_float2(rstd, rstd), g2, make_float2(add[j], add[j + 1]));
-                        gw[at][j] = o2.x, gw[at][j + 1] = o2.y;
-                    }
+                for (int j = 0; j < VEC; j += 2) {
+                    const float2 g2 = __ffma2_rn(make_float2(-mean, -mean), make_float2(xh[at][j], xh[at][j + 1]), make_float2(gw[at][j], gw[at][j + 1]));
+                    const float2 o2 = __ffma2_rn(make_float2(rstd, rstd), g2, make_float2(add[j], add[j + 1]));
+                    gw[at][j] = o2.x, gw[at][j + 1] = o2.y;
                 }
                 store_raw<T, VEC>(static_cast<T *>(p.dx) + base + c, gw[at]);
             }
@@ -591,12 +562,8 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
     for (int i = 0; i < NV; ++i) {
         const int c = (threadIdx.x + i * blockDim.x) * VEC;
         if (c < p.K) {
-            if constexpr (VEC >= 4) {
 #pragma unroll
-                for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4 *>(mine + c + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
-            } else {
-                mine[c] = dw[i][0];
-            }
+            for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4 *>(mine + c + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
         }
     }
     if (groups > 1) {
@@ -606,6 +573,76 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
             float sum = 0.0f;
             for (int g = 0; g < groups; ++g) sum += all[(size_t)g * (blockDim.x * NV * VEC) + c];
             to[c] = sum;
+        }
+    }
+}
+
+// Rows that are no whole vectors, or buffers that do not start on 16 bytes: element by element through registers, one row ahead.  (Through
+// the ring 1003 x 1509 of fp32 took 12.7 us instead of 9, 8192 x 1021 of bf16 39 instead of 30.)
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024)
+esmm_rmsnorm_backward_ragged_kernel(const NormGradParams p)
+{
+    grid_launch_dependents();
+    grid_dependency_wait();
+    __shared__ float slots[64];
+    const T *weight = static_cast<const T *>(p.weight);
+    const T *dout = static_cast<const T *>(p.dout), *h = static_cast<const T *>(p.h), *dsum = static_cast<const T *>(p.dsum);
+    float dw[NV];
+    T w[NV], g_raw[NV], h_raw[NV], s_raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
+        dw[i] = 0.0f;
+        w[i] = weight && c < p.K ? weight[c] : from_float<T>(1.0f);
+    }
+    float rstd_next = 0.0f;
+    auto load_row = [&](size_t row) {
+        const size_t base = row * (size_t)p.K;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c < p.K) {
+                g_raw[i] = dout[base + c];
+                h_raw[i] = h[base + c];
+                if (dsum) s_raw[i] = dsum[base + c];
+            }
+        }
+        rstd_next = p.rstd[row];
+    };
+    load_row(blockIdx.x);
+    int turn = 0;
+    for (size_t row = blockIdx.x; row < (size_t)p.M; row += gridDim.x, turn ^= 32) {
+        const size_t base = row * (size_t)p.K;
+        const float rstd = rstd_next;
+        float gw[NV], xh[NV], add[NV], dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            gw[i] = xh[i] = add[i] = 0.0f;
+            if (threadIdx.x + i * blockDim.x < (unsigned)p.K) {
+                const float g = to_float<T>(g_raw[i]);
+                xh[i] = to_float<T>(h_raw[i]) * rstd;
+                if (dsum) add[i] = to_float<T>(s_raw[i]);
+                dw[i] = fmaf(g, xh[i], dw[i]);
+                gw[i] = g * to_float<T>(w[i]);
+                dot = fmaf(gw[i], xh[i], dot);
+            }
+        }
+        if (row + gridDim.x < (size_t)p.M) load_row(row + gridDim.x);
+        // (two sets of slots in turn: a warp may be a row ahead of the slowest one's reads)
+        const float mean = row_reduce<false>(dot, slots + turn) / (float)p.K;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c < p.K && bounds_ok(base + c < (size_t)p.M * p.K, p.status, 62))
+                static_cast<T *>(p.dx)[base + c] = from_float<T>(fmaf(rstd, fmaf(-mean, xh[i], gw[i]), add[i]));
+        }
+    }
+    if (p.partial) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = threadIdx.x + i * blockDim.x;
+            if (c < p.K) p.partial[(size_t)blockIdx.x * p.K + c] = dw[i];
         }
     }
 }
@@ -899,37 +936,47 @@ static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas
 {
     constexpr int VEC = 16 / (int)sizeof(T);
     const bool vectors = aligned && p.K % VEC == 0;
-    p.row_bytes = ceil_div(p.K * (int)sizeof(T), 16) * 16 + (vectors ? 0 : 16);
-    auto go = [&](auto tag, auto nv, auto most, auto keep) -> int {
-        constexpr int V = decltype(tag)::value, N = decltype(nv)::value;
-        constexpr auto kernel = &esmm_rmsnorm_backward_kernel<T, V, N, decltype(most)::value, decltype(keep)::value != 0>;
-        const int threads = ceil_div(ceil_div(p.K, V * N), 32) * 32;
+    p.row_bytes = p.K * (int)sizeof(T);
+    auto go = [&](auto nv, auto most, auto keep) -> int {
+        constexpr int N = decltype(nv)::value;
+        constexpr auto kernel = &esmm_rmsnorm_backward_kernel<T, VEC, N, decltype(most)::value, decltype(keep)::value != 0>;
+        const int threads = ceil_div(ceil_div(p.K, VEC * N), 32) * 32;
         const int groups = threads == 32 ? std::min(4, p.M) : 1;
         // As many rows under way as the SM's shared memory holds, two per group at least, in one to four CTAs per SM.  More CTAs leave
         // more partial rows of dw to add up; they pay for short rows where each has many (one / two / four CTAs per SM, us: 8192 x 4096
-        // bf16 67 / 46 / 52, 8192 x 1021 bf16 104 / 60 / 40, 1003 x 1509 fp32 16.9 / 12.7 / 15.3, 4096 x 4096 fp32 45 / 48.5 / 48.5).
+        // bf16 67 / 46 / 52, 8192 x 1024 fp32 60 / 35 / 28, 4096 x 4096 fp32 45 / 48.5 / 48.5).
         int per_sm = threads > 256 ? 1 : threads <= 128 && groups == 1 && p.M >= 32 * sms ? 4 : 2;
         while (per_sm > 1 && RING_BYTES / per_sm < 2 * groups * 3 * p.row_bytes) --per_sm;
         *ctas = std::max(1, std::min(std::min(ceil_div(p.M, groups), ROWS_MAX_PARTIALS), sms * per_sm));
         p.stages = std::max(1, std::min({8, RING_BYTES / per_sm / (groups * 3 * p.row_bytes), ceil_div(p.M, *ctas * groups)}));
         // (the groups' sums of dw are added up where the rings were)
-        const size_t smem = std::max((size_t)groups * p.stages * (3 * p.row_bytes + 8), groups > 1 ? (size_t)groups * threads * N * V * 4 : 0);
+        p.bar_off = std::max(groups * p.stages * 3 * p.row_bytes, groups > 1 ? groups * threads * N * VEC * 4 : 0);
+        const size_t smem = (size_t)p.bar_off + groups * p.stages * 8;
         const int st = allow_ring<kernel>();
         if (st != ESMM_OK) return st;
         ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads, groups), smem, stream, p));
         return ESMM_OK;
     };
-    if (aligned && 2 * 3 * p.row_bytes <= RING_BYTES) {
-        if (vectors && p.K <= 32 * VEC) return go(Num<VEC>(), Num<1>(), Num<128>(), Num<1>());
-        if (vectors && p.K <= 64 * VEC) return go(Num<VEC>(), Num<2>(), Num<128>(), Num<1>());
-        if (vectors && VEC == 8 && p.K <= 128 * VEC) return go(Num<VEC>(), Num<4>(), Num<128>(), Num<1>());
-        if (vectors && p.K <= 512 * VEC) return go(Num<VEC>(), Num<2>(), Num<256>(), Num<1>());
-        if (vectors && p.K <= 1024 * VEC) return go(Num<VEC>(), Num<2>(), Num<512>(), Num<1>());
-        if (vectors && p.K <= 2048 * VEC) return go(Num<VEC>(), Num<4>(), Num<512>(), Num<0>());
-        if (!vectors && p.K <= 128) return go(Num<1>(), Num<4>(), Num<128>(), Num<1>());
-        if (!vectors && p.K <= 4096) return go(Num<1>(), Num<8>(), Num<512>(), Num<1>());
-        if (!vectors && p.K <= 8192) return go(Num<1>(), Num<8>(), Num<1024>(), Num<0>());
+    if (vectors && 2 * 3 * p.row_bytes <= RING_BYTES) {
+        if (p.K <= 32 * VEC) return go(Num<1>(), Num<128>(), Num<1>());
+        if (p.K <= 64 * VEC) return go(Num<2>(), Num<128>(), Num<1>());
+        if (VEC == 8 && p.K <= 128 * VEC) return go(Num<4>(), Num<128>(), Num<1>());
+        if (p.K <= 512 * VEC) return go(Num<2>(), Num<256>(), Num<1>());
+        if (p.K <= 1024 * VEC) return go(Num<2>(), Num<512>(), Num<1>());
+        if (p.K <= 2048 * VEC) return go(Num<4>(), Num<512>(), Num<0>());
     }
+    auto ragged = [&](auto nv) -> int {
+        constexpr int N = decltype(nv)::value;
+        auto *kernel = esmm_rmsnorm_backward_ragged_kernel<T, N>;
+        const int threads = ceil_div(ceil_div(p.K, N), 32) * 32;
+        int per_sm = 0;
+        ESMM_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0));
+        *ctas = std::max(1, std::min(std::min(p.M, ROWS_MAX_PARTIALS), sms * std::max(1, std::min(per_sm, 4))));
+        ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads), 0, stream, p));
+        return ESMM_OK;
+    };
+    if (!vectors && p.K <= 1024 * 2) return ragged(Num<4>());
+    if (!vectors && p.K <= 1024 * 8) return ragged(Num<8>());
     *ctas = std::max(1, std::min(std::min(p.M, ROWS_MAX_PARTIALS), 2 * sms));
     ESMM_CUDA_TRY(launch_dependent(esmm_rmsnorm_backward_long_kernel<T>, dim3((unsigned)*ctas), dim3(1024), 0, stream, p));
     return ESMM_OK;

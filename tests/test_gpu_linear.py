@@ -78,6 +78,16 @@ def test_e4m3_kernels(cuda, pkg, tuning, pair):
         check(pkg, m, n, k, "e4m3", out="bf16", activation="gelu_tanh", bias=True, residual=True, pre=True, scales=True)
 
 
+@pytest.mark.parametrize("pair,tail", [(128, 64), (192, 64), (192, 128), (256, 64), (256, 128), (256, 192)])
+def test_two_tile_widths(cuda, pkg, tuning, pair, tail):
+    tuning("LINEAR_PAIR", pair)
+    tuning("LINEAR_TAIL", tail)
+    for trans in ("nn", "nt", "tn"):
+        check(pkg, 520, 1512, 200, "bf16", trans_a=trans == "tn", trans_b=trans == "nt", activation="silu", bias=True, residual=True, pre=True)
+    check(pkg, 300, 2056, 400, "e4m3", out="f16", bias=True, residual=True, scales=True)
+    check(pkg, 9, pair + 8, 64, "f16", bias=True)
+
+
 @pytest.mark.parametrize("split", [1, 2, 3, 8])
 @pytest.mark.parametrize("columns", [64, 128])
 def test_parts_of_k(cuda, pkg, tuning, split, columns):
