@@ -241,24 +241,23 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     const bool leader = rank == 0;
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {                                           // a barrier per lane
+        if (lane < p.stages) {
+            mbar_init(full0 + 8 * lane, 1);                    // (even CTA) its producers; bytes of both CTAs' copies
+            mbar_init(empty0 + 8 * lane, 1);                   // one commit per stage, delivered to both CTAs
+        } else if (lane >= 16 && lane < 16 + LP_EPI_WARPS) {
+            mbar_init(res0 + 8 * (lane - 16), 1);
+        } else if (lane >= 24 && lane < 26) {
+            mbar_init(accf0 + 8 * (lane - 24), 1);
+            mbar_init(acce0 + 8 * (lane - 24), 2 * LP_EPI_WARPS);   // (even CTA) the epilogue warps of both CTAs
+        }
+        if (lane == 26) *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    } else if (warp == 1 && lane == 0) {
         tma_prefetch_descriptor(&maps.a);
         tma_prefetch_descriptor(&maps.b[0]);
         tma_prefetch_descriptor(&maps.c);
-    }
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full0 + 8 * s, 1);                   // (even CTA) its producer; bytes of both CTAs' copies
-            mbar_init(empty0 + 8 * s, 1);                  // one commit per stage, delivered to both CTAs
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(accf0 + 8 * b, 1);
-            mbar_init(acce0 + 8 * b, 2 * LP_EPI_WARPS);    // (even CTA) the epilogue warps of both CTAs
-        }
-        for (int w = 0; w < LP_EPI_WARPS; ++w) mbar_init(res0 + 8 * w, 1);
-        *abort_flag = 0;
-        fence_barrier_init();
-        fence_proxy_async();
     }
     if (warp == L_PRODUCERS) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -586,13 +585,14 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             linear_prefetch(&maps.b[0], p.b_k_major ? k : r, p.b_k_major ? r : k);
         }
     }
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 1);
+    if (warp == 0) {
+        if (lane < p.stages) {
+            mbar_init(full0 + 8 * lane, 1);
+            mbar_init(empty0 + 8 * lane, 1);
+        } else if (lane == 31) {
+            mbar_init(accf, 1);
+            *abort_flag = 0;
         }
-        mbar_init(accf, 1);
-        *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
@@ -755,7 +755,7 @@ struct LinearChoice {
 
 // Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
 // shapes (M = 1 .. 2048; K and N from 512 to 11008; 16 and 8 bits, B 0.25 to 90 MB, three sets of operands in turn): what the rule picks takes
-// 1.5 % longer than the best variant on average, 18 % at most.
+// 1.0 % longer than the best variant on average, 14 % at most.  (What all variants have in common, about 3 us, is left out.)
 static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
 {
     LinearChoice c = {0, 0, 0, 128, 1};
@@ -764,12 +764,12 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
     double best = 1e30;
     // a K step: the MMAs, or the copies, which are slower the more SMs copy
     auto step = [&](int nb, long tiles) {
-        return std::max(nb * 0.00127, (256 + nb) * (0.000256 + 0.0003 * (double)std::min<long>(tiles, pairs) / pairs));
+        return std::max(nb * 0.00156, (256 + nb) * (0.000396 + 0.000246 * (double)std::min<long>(tiles, pairs) / pairs));
     };
     for (int nb = 64; nb <= 256; nb += 64) {
         const int across = ceil_div(N, nb);
         const long tiles = (long)down * across, rounds = (tiles + pairs - 1) / pairs;
-        const double fixed = 3.9 + 0.68 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm);
+        const double fixed = 0.62 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm) + 0.62 * (rounds - 1);
         if (t < best) best = t, c.pair_nb = nb, c.columns = c.tail_nb = 0;
         // where the last round is partly filled: whole rounds of this width, the columns that are left in narrower tiles
         const int columns = (int)std::min<long>(across, tiles / pairs * pairs / down);
@@ -777,7 +777,7 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
         for (int tail = 64; tail < nb; tail += 64) {
             const long first = (long)columns * down, all = first + (long)ceil_div(N - columns * nb, tail) * down;
             const long wide = (first + pairs - 1) / pairs, narrow = (all + pairs - 1) / pairs - wide;
-            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm);
+            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 0.62 * (wide + narrow - 1);
             if (tt < 0.98 * best) best = tt, c.pair_nb = nb, c.tail_nb = tail, c.columns = columns;
         }
     }
@@ -789,11 +789,11 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
             const long ctas = tiles * split, rounds = (ctas + 2 * sms - 1) / (2 * sms);
             const int steps = ceil_div(ksteps, split);
             const double kb = (box + nb) * (L_KBYTES / 1000.0);                // copied per step and CTA
-            const double one = rounds * steps * std::max(0.179, kb / 82.6), all = ctas * steps * kb / 17700.0;
+            const double one = rounds * steps * std::max(0.191, kb / 67.7), all = ctas * steps * kb / 15350.0;
             // (fewer CTAs than the SMs have room for have less of HBM under way)
             const double bytes = hbm * (1.0 + 0.5 * (1.0 - (double)ctas / (rounds * 2 * sms)));
-            const double t = 3.2 + 2.6 * rows * nb / 16384 + std::max({one, all, bytes}) + 1.8 * (rounds - 1) +
-                             (split - 1) * (0.077 + (double)M * N * 4 / 3.46e6);   // sums through distributed shared memory
+            const double t = 0.58 + 0.82 * rows * nb / 16384 + std::max({one, all, bytes}) + 0.06 * (rounds - 1) + 0.93 * ctas / (2 * sms) +
+                             (split - 1) * (0.03 + (double)M * N * 4 / 3.32e6);   // sums through distributed shared memory
             if (t < best) best = t, c = {0, 0, 0, nb, split};
         }
     }
@@ -909,7 +909,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
         p.slot_bytes = p.kind[0].stage_bytes;
         // One box per epilogue warp leaves room for a sixth stage of the widest tiles, which long K gains from; with short K the epilogue's own
         // time counts, and the next piece's residual is under way in the second box.
-        p.boxes = tuning_get("STAGES", 0) ? tuning_get("STAGES", 0) : p.ksteps >= 16 ? 1 : 2;
+        p.boxes = p.ksteps >= 16 ? 1 : 2;
         const int staging = LP_EPI_WARPS * p.boxes * LP_BOX;
         p.stages = std::min(LP_MAX_STAGES, (LP_COLUMN_OFF - staging) / p.slot_bytes);
         p.box_off = LP_COLUMN_OFF - staging;
