@@ -483,10 +483,13 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
 // ----------------------------------------------------------------------------------------------------------------------------
 // Split kernel
 // ----------------------------------------------------------------------------------------------------------------------------
-constexpr int LS_DRAIN_WARPS = 8;                 // half the accumulator's columns each; then a warp that copies and one that issues the MMAs
+constexpr int LS_DRAIN_WARPS = 8;                 // half the accumulator's columns each; then warps that copy and one that issues the MMAs
 constexpr int LS_THREADS = (LS_DRAIN_WARPS + L_PRODUCERS + 1) * 32;
 constexpr int LS_MAX_STAGES = 16;
 constexpr int LS_MAX_SPLIT = 8;
+// At least so much shared memory per CTA, so that no more than four are on an SM: tensor memory has room for the accumulators of four, and
+// a CTA that waited for it would hold up the rest of its cluster.
+constexpr int LS_MIN_SMEM = 50 * 1024;
 
 // shared memory: ring of A, ring of B (the sums lie over both after the last MMA) | barriers, flags
 __host__ __device__ constexpr int ls_red_bytes(int rows, int nb) { return rows * (nb + 4) * 4; }
@@ -678,7 +681,6 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
     __syncwarp();
     linear_cluster_sync();       // all parts' sums are in their CTAs' shared memory
 
-    // Eight outputs of a row at a time: the parts' sums in the order of K, the epilogue, one 16-byte store.
     uint32_t part_base[LS_MAX_SPLIT];
 #pragma unroll
     for (int part = 0; part < LS_MAX_SPLIT; ++part)
@@ -825,6 +827,8 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     if (trans_a && trans_b) return ESMM_ERR_UNSUPPORTED;
     if (!activation_known(activation)) return ESMM_ERR_UNSUPPORTED;
     if (M <= 0 || N <= 0 || K <= 0 || N % 8) return ESMM_ERR_SHAPE;
+    constexpr int most = 0x7FFFFFFF - 65536;   // (rows, columns and k are counted in int, in steps of tiles)
+    if (M > most || N > most || K > most) return ESMM_ERR_TOO_LARGE;
     // rows of 16 bytes: A's are K (or, transposed, M) long, B's N or K
     const int per16 = f8 ? 16 : 8;
     if ((trans_a ? M : K) % per16 || (trans_b ? K % per16 : 0)) return ESMM_ERR_SHAPE;
@@ -932,7 +936,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     p.stages = std::max(p.stages, ceil_div(128 * L_KBYTES, b_stage));
     const int ring = p.stages * (p.a_stage_bytes + b_stage);
     const int bar_off = (std::max(ring, ls_red_bytes(std::min(M, 128), choice.nb)) + 15) & ~15;
-    const size_t smem = (size_t)bar_off + (2 * LS_MAX_STAGES + 1) * 8 + 16;
+    const size_t smem = std::max((size_t)bar_off + (2 * LS_MAX_STAGES + 1) * 8 + 16, (size_t)LS_MIN_SMEM);
     if (smem > (size_t)SMEM_LIMIT) return ESMM_ERR_TOO_LARGE;
     auto go = [&](auto kernel) -> int {
         cudaLaunchConfig_t cfg = {};

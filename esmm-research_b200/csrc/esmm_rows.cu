@@ -911,6 +911,9 @@ static int norm_launch(const NormParams &p, int dtype, bool out8, bool aligned, 
 
 template <int N> struct Num { static constexpr int value = N; };
 
+// Rows and columns are counted in int, in steps of up to a CTA's threads.
+constexpr int MAX_EXTENT = 0x7FFFFFFF - 65536;
+
 static bool row_dtype(int dtype) { return dtype == ESMM_F32 || dtype == ESMM_F16 || dtype == ESMM_BF16; }
 
 static bool element_aligned(const void *p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
@@ -936,7 +939,7 @@ static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas
 {
     constexpr int VEC = 16 / (int)sizeof(T);
     const bool vectors = aligned && p.K % VEC == 0;
-    p.row_bytes = p.K * (int)sizeof(T);
+    p.row_bytes = p.K <= 2048 * VEC ? p.K * (int)sizeof(T) : 0;
     auto go = [&](auto nv, auto most, auto keep) -> int {
         constexpr int N = decltype(nv)::value;
         constexpr auto kernel = &esmm_rmsnorm_backward_kernel<T, VEC, N, decltype(most)::value, decltype(keep)::value != 0>;
@@ -957,13 +960,13 @@ static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas
         ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads, groups), smem, stream, p));
         return ESMM_OK;
     };
-    if (vectors && 2 * 3 * p.row_bytes <= RING_BYTES) {
+    if (vectors && p.K <= 2048 * VEC && 2 * 3 * p.row_bytes <= RING_BYTES) {
         if (p.K <= 32 * VEC) return go(Num<1>(), Num<128>(), Num<1>());
         if (p.K <= 64 * VEC) return go(Num<2>(), Num<128>(), Num<1>());
         if (VEC == 8 && p.K <= 128 * VEC) return go(Num<4>(), Num<128>(), Num<1>());
         if (p.K <= 512 * VEC) return go(Num<2>(), Num<256>(), Num<1>());
         if (p.K <= 1024 * VEC) return go(Num<2>(), Num<512>(), Num<1>());
-        if (p.K <= 2048 * VEC) return go(Num<4>(), Num<512>(), Num<0>());
+        return go(Num<4>(), Num<512>(), Num<0>());
     }
     auto ragged = [&](auto nv) -> int {
         constexpr int N = decltype(nv)::value;
@@ -1004,6 +1007,7 @@ int esmm_rmsnorm(int M, int K, int dtype, const void *d_x, const void *d_residua
     const bool out8 = out_dtype == ESMM_E4M3;
     if (!d_x || !d_out || (out8 && !d_scale)) return ESMM_ERR_NULL;
     if (M <= 0 || K <= 0) return ESMM_ERR_SHAPE;
+    if (M > MAX_EXTENT || K > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
     if (!row_dtype(dtype) || (!out8 && out_dtype != dtype)) return ESMM_ERR_UNSUPPORTED;
     const int size = dtype_bytes(dtype);
     for (const void *q : {d_x, d_residual, d_weight, (const void *)d_sum, (const void *)(out8 ? nullptr : d_out)})
@@ -1031,6 +1035,7 @@ int esmm_quantize_rows(int M, int K, int dtype, const void *d_x, void *d_out, fl
     using namespace esmm;
     if (!d_x || !d_out || !d_scale) return ESMM_ERR_NULL;
     if (M <= 0 || K <= 0) return ESMM_ERR_SHAPE;
+    if (M > MAX_EXTENT || K > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
     if (!row_dtype(dtype)) return ESMM_ERR_UNSUPPORTED;
     const int size = dtype_bytes(dtype);
     if (!element_aligned(d_x, size) || !element_aligned(d_scale, 4)) return ESMM_ERR_ALIGN;
@@ -1059,6 +1064,7 @@ int esmm_rmsnorm_backward(int M, int K, int dtype, const void *d_dout, const voi
     cudaStream_t stream = (cudaStream_t)stream_;
     if (!d_dout || !d_h || !d_rstd || !d_dx || (d_dweight && !d_workspace)) return ESMM_ERR_NULL;
     if (M <= 0 || K <= 0) return ESMM_ERR_SHAPE;
+    if (M > MAX_EXTENT || K > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
     if (!row_dtype(dtype)) return ESMM_ERR_UNSUPPORTED;
     const int size = dtype_bytes(dtype);
     for (const void *q : {d_dout, d_h, d_weight, d_dsum, (const void *)d_dx, (const void *)d_dweight})
@@ -1104,6 +1110,7 @@ int esmm_epilogue_backward(int M, int N, int dtype, const void *d_dC, const void
     if (!row_dtype(dtype) || !activation_known(activation)) return ESMM_ERR_UNSUPPORTED;
     const int vec = 16 / dtype_bytes(dtype);
     if (M <= 0 || N <= 0 || N % vec) return ESMM_ERR_SHAPE;
+    if (M > MAX_EXTENT || N > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
     if (!aligned16({d_dC, d_pre, d_dZ, d_workspace}) || !element_aligned(d_dbias, dtype_bytes(dtype))) return ESMM_ERR_ALIGN;
     EpiGradParams p;
     memset(&p, 0, sizeof p);
@@ -1143,7 +1150,7 @@ int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float 
     if (K <= 0 || N <= 0 || K % 16) return ESMM_ERR_SHAPE;
     if (!row_dtype(dtype)) return ESMM_ERR_UNSUPPORTED;
     if (!element_aligned(d_B, dtype_bytes(dtype)) || ((uintptr_t)d_bt & 15) || !element_aligned(d_scale, 4)) return ESMM_ERR_ALIGN;
-    if (ceil_div(K, 128) > 65535) return ESMM_ERR_TOO_LARGE;
+    if (K / 128 >= 65535 || N > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
     auto go = [&](auto tag) -> int {
         typedef decltype(tag) T;
         const T *B = static_cast<const T *>(d_B);

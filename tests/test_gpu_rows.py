@@ -253,3 +253,69 @@ def test_feed_forward_block_in_8_bits(cuda, pkg, m):
     _, want, mag = d.linear(q2.double(), bt2.double().t(), r2, s2, None, "none", h)
     off = d.sum_error(mag, n) + 2.0 ** -20 * want.abs()
     d.assert_close(out, want, off + ub * (want.abs() + off))
+
+
+def test_norm_captured_and_replayed_with_new_inputs(cuda, pkg):
+    m, k = 300, 1032
+    sets = [tensors(m, k, "bf16", seed=s) for s in (11, 12)]
+    x, res, w, dout, dsum = (v.clone() for v in sets[0])
+    h, out, dx = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    q, scale, rstd = torch.empty((m, k), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    dw = torch.empty_like(w)
+    ws = torch.empty(pkg.rmsnorm_backward_workspace_bytes(m, k), dtype=torch.uint8, device="cuda")
+
+    def calls(stream):
+        pkg.rmsnorm(m, k, pkg.BF16, x.data_ptr(), res.data_ptr(), w.data_ptr(), EPS, h.data_ptr(), pkg.BF16, out.data_ptr(), 0, rstd.data_ptr(), stream)
+        pkg.rmsnorm_backward(m, k, pkg.BF16, dout.data_ptr(), h.data_ptr(), w.data_ptr(), rstd.data_ptr(), dsum.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+                             ws.data_ptr(), stream)
+        pkg.quantize_rows(m, k, pkg.BF16, out.data_ptr(), q.data_ptr(), scale.data_ptr(), stream)
+    outputs = (h, out, rstd, dx, dw, q.view(torch.uint8), scale)
+    want = []
+    for s in sets:
+        for to, v in zip((x, res, w, dout, dsum), s):
+            to.copy_(v)
+        calls(0)
+        torch.cuda.synchronize()
+        want.append([o.clone() for o in outputs])
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        calls(torch.cuda.current_stream().cuda_stream)
+    for s, expected in zip(sets, want):
+        for to, v in zip((x, res, w, dout, dsum), s):
+            to.copy_(v)
+        for o in outputs:
+            o.zero_()
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outputs, expected):
+            assert torch.equal(o, e)
+    pkg.device_status()
+
+
+def test_norms_on_two_streams_at_once(cuda, pkg):
+    m, k = 700, 2048
+    runs = []
+    for seed in (21, 22):
+        x, res, w, dout, dsum = tensors(m, k, "bf16", seed=seed)
+        runs.append(dict(x=x, res=res, w=w, dout=dout, dsum=dsum, h=torch.empty_like(x), out=torch.empty_like(x), dx=torch.empty_like(x), dw=torch.empty_like(w),
+                         rstd=torch.empty(m, device="cuda"), ws=torch.empty(pkg.rmsnorm_backward_workspace_bytes(m, k), dtype=torch.uint8, device="cuda"),
+                         stream=torch.cuda.Stream()))
+
+    def go(r, stream):
+        p = {key: v.data_ptr() for key, v in r.items() if key != "stream"}
+        pkg.rmsnorm(m, k, pkg.BF16, p["x"], p["res"], p["w"], EPS, p["h"], pkg.BF16, p["out"], 0, p["rstd"], stream)
+        pkg.rmsnorm_backward(m, k, pkg.BF16, p["dout"], p["h"], p["w"], p["rstd"], p["dsum"], p["dx"], p["dw"], p["ws"], stream)
+    want = []
+    for r in runs:
+        go(r, 0)
+        torch.cuda.synchronize()
+        want.append([r[key].clone() for key in ("h", "out", "dx", "dw")])
+    for _ in range(20):
+        for r in runs:
+            go(r, r["stream"].cuda_stream)
+    torch.cuda.synchronize()
+    pkg.device_status()
+    for r, e in zip(runs, want):
+        for key, v in zip(("h", "out", "dx", "dw"), e):
+            assert torch.equal(r[key], v)
