@@ -494,74 +494,111 @@ constexpr int LS_MIN_SMEM = 50 * 1024;
 // shared memory: ring of A, ring of B (the sums lie over both after the last MMA) | barriers, flags
 __host__ __device__ constexpr int ls_red_bytes(int rows, int nb) { return rows * (nb + 4) * 4; }
 
-// The share of CTA `rank` of a tile's outputs: four columns per thread and row, neighbouring threads on neighbouring columns (reads of
-// the other CTAs' sums move 16 bytes per lane without gaps), a few rows at a time so that their loads are under way together.
-// part_base: the sums in each CTA of the cluster (obtained after the cluster barrier, so that no load from them can be moved before it).
-template <int NB, int SPLIT>
-__device__ __forceinline__ void linear_split_finish(const LinearParams &p, const uint32_t (&part_base)[LS_MAX_SPLIT], int rank, int row0, int col0, int rows)
-{
-    constexpr int LANES = NB / 4, ROWS = LS_THREADS / LANES, U = SPLIT == 1 ? 4 : SPLIT <= 4 ? 2 : 1;
-    const int c = (threadIdx.x % LANES) * 4, col = col0 + c;
-    if (col >= p.N) return;
-    auto unpack2 = [&](uint32_t w) { return p.bf16 ? unpack_bf16(w) : unpack_f16(w); };
-    auto pack2 = [&](float lo, float hi) { return p.bf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); };
-    float bias[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {1.f, 1.f, 1.f, 1.f};
-    if (p.bias) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.bias) + (size_t)col * 2);
-        const float2 f0 = unpack2(w.x), f1 = unpack2(w.y);
-        bias[0] = f0.x, bias[1] = f0.y, bias[2] = f1.x, bias[3] = f1.y;
-    }
-    if (p.b_scale) {   // (aligned to its elements only)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sb[j] = p.b_scale[col + j];
-    }
-    for (int r = rank * ROWS + threadIdx.x / LANES; r < rows; r += SPLIT * ROWS * U) {
-        float4 u[U][SPLIT];
-        uint2 res[U];
-        float sa[U];
+// The share of CTA `rank` of a tile's outputs, by the draining warps: four columns per thread and row, neighbouring threads on neighbouring
+// columns (reads of the other CTAs' sums move 16 bytes per lane without gaps), a few rows at a time so that their loads are under way
+// together.  What the epilogue reads beside the sums is fetched before the last MMA: the column's scale and bias, and for the thread's
+// first rows the row's scale and the residual.
+template <int NB>
+struct LinearSplitEpilogue {
+    static constexpr int LANES = NB / 4, ROWS = LS_DRAIN_WARPS * 32 / LANES, U = 2;
+    float bias[4], sb[4];
+    float sa[U];
+    uint2 res[U];
+
+    __device__ __forceinline__ static float2 unpack2(const LinearParams &p, uint32_t w) { return p.bf16 ? unpack_bf16(w) : unpack_f16(w); }
+    __device__ __forceinline__ static uint32_t pack2(const LinearParams &p, float lo, float hi) { return p.bf16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); }
+
+    // rows r, r + step, ...
+    __device__ __forceinline__ void fetch_rows(const LinearParams &p, int row0, int col, int r, int step, int rows)
+    {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int ri = r + i * SPLIT * ROWS;
-            if (ri >= rows) break;
-#pragma unroll
-            for (int part = 0; part < SPLIT; ++part) {
-                const uint32_t at = part_base[part] + (uint32_t)((ri * (NB + 4) + c) * 4);
-                if constexpr (SPLIT == 1)
-                    asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
-                else
-                    asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+            const int ri = r + i * step;
+            sa[i] = 1.0f;
+            if (ri < rows) {
+                if (p.a_scale) sa[i] = p.a_scale[row0 + ri];
+                if (p.has_residual) res[i] = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.residual) + ((size_t)(row0 + ri) * p.N + col) * 2);
             }
-            const size_t off = (size_t)(row0 + ri) * p.N + col;
-            if (p.has_residual) res[i] = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.residual) + off * 2);
-            sa[i] = p.a_scale ? p.a_scale[row0 + ri] : 1.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int ri = r + i * SPLIT * ROWS;
-            if (ri >= rows) break;
-            const size_t off = (size_t)(row0 + ri) * p.N + col;
-            float z[4] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w};
-#pragma unroll
-            for (int part = 1; part < SPLIT; ++part) z[0] += u[i][part].x, z[1] += u[i][part].y, z[2] += u[i][part].z, z[3] += u[i][part].w;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) z[j] = fmaf(z[j] * sa[i], sb[j], bias[j]);
-            const bool inside = bounds_ok(off + 4 <= (size_t)p.M * p.N, p.status, 64);   // checked build: site 64
-            if (p.has_pre && inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.pre) + off * 2) = make_uint2(pack2(z[0], z[1]), pack2(z[2], z[3]));
-            with_activation(p.activation, [&](auto tag) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
-            });
-            if (p.has_residual) {
-                const float2 f0 = unpack2(res[i].x), f1 = unpack2(res[i].y);
-                z[0] += f0.x, z[1] += f0.y, z[2] += f1.x, z[3] += f1.y;
-            }
-            if (inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.C) + off * 2) = make_uint2(pack2(z[0], z[1]), pack2(z[2], z[3]));
         }
     }
-}
+
+    __device__ __forceinline__ void fetch(const LinearParams &p, int rank, int split, int row0, int col0, int rows)
+    {
+        const int col = col0 + (threadIdx.x % LANES) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bias[j] = 0.0f, sb[j] = 1.0f;
+        if (col >= p.N) return;
+        if (p.bias) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const char *>(p.bias) + (size_t)col * 2);
+            const float2 f0 = unpack2(p, w.x), f1 = unpack2(p, w.y);
+            bias[0] = f0.x, bias[1] = f0.y, bias[2] = f1.x, bias[3] = f1.y;
+        }
+        if (p.b_scale) {   // (aligned to its elements only)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sb[j] = p.b_scale[col + j];
+        }
+        fetch_rows(p, row0, col, rank * ROWS + threadIdx.x / LANES, split * ROWS, rows);
+    }
+
+    // sums: this CTA's, at the same place in every CTA of the cluster
+    template <int SPLIT>
+    __device__ __forceinline__ void finish(const LinearParams &p, uint32_t sums, int rank, int row0, int col0, int rows)
+    {
+        // (obtained after the cluster barrier, so that no load from them can be moved before it)
+        uint32_t part_base[SPLIT];
+#pragma unroll
+        for (int part = 0; part < SPLIT; ++part) part_base[part] = SPLIT == 1 ? sums : linear_map_to_cta(sums, (uint32_t)part);
+        constexpr int V = SPLIT <= 2 ? U : SPLIT <= 4 ? 2 : 1;      // rows whose sums are loaded together
+        const int c = (threadIdx.x % LANES) * 4, col = col0 + c;
+        if (col >= p.N) return;
+        const int first = rank * ROWS + threadIdx.x / LANES;
+        for (int r = first; r < rows; r += SPLIT * ROWS * U) {
+            if (r != first) fetch_rows(p, row0, col, r, SPLIT * ROWS, rows);
+#pragma unroll
+            for (int i0 = 0; i0 < U; i0 += V) {
+                float4 u[V][SPLIT];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int ri = r + (i0 + i) * SPLIT * ROWS;
+                    if (ri >= rows) break;
+#pragma unroll
+                    for (int part = 0; part < SPLIT; ++part) {
+                        const uint32_t at = part_base[part] + (uint32_t)((ri * (NB + 4) + c) * 4);
+                        if constexpr (SPLIT == 1)
+                            asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+                        else
+                            asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int ri = r + (i0 + i) * SPLIT * ROWS;
+                    if (ri >= rows) break;
+                    const size_t off = (size_t)(row0 + ri) * p.N + col;
+                    float z[4] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w};
+#pragma unroll
+                    for (int part = 1; part < SPLIT; ++part) z[0] += u[i][part].x, z[1] += u[i][part].y, z[2] += u[i][part].z, z[3] += u[i][part].w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) z[j] = fmaf(z[j] * sa[i0 + i], sb[j], bias[j]);
+                    const bool inside = bounds_ok(off + 4 <= (size_t)p.M * p.N, p.status, 64);   // checked build: site 64
+                    if (p.has_pre && inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.pre) + off * 2) = make_uint2(pack2(p, z[0], z[1]), pack2(p, z[2], z[3]));
+                    with_activation(p.activation, [&](auto tag) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
+                    });
+                    if (p.has_residual) {
+                        const float2 f0 = unpack2(p, res[i0 + i].x), f1 = unpack2(p, res[i0 + i].y);
+                        z[0] += f0.x, z[1] += f0.y, z[2] += f1.x, z[3] += f1.y;
+                    }
+                    if (inside) *reinterpret_cast<uint2 *>(static_cast<char *>(p.C) + off * 2) = make_uint2(pack2(p, z[0], z[1]), pack2(p, z[2], z[3]));
+                }
+            }
+        }
+    }
+};
 
 template <int NB, bool F8>
-__global__ void __launch_bounds__(LS_THREADS)
+__global__ void __launch_bounds__(LS_THREADS, 2)
 esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p, const int split, const int bar_off)
 {
     extern __shared__ __align__(1024) char smem[];
@@ -588,6 +625,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             linear_prefetch(&maps.b[0], p.b_k_major ? k : r, p.b_k_major ? r : k);
         }
     }
+    if (warp == 1 && lane == 0) tma_prefetch_descriptor(&maps.a);
     if (warp == 0) {
         if (lane < p.stages) {
             mbar_init(full0 + 8 * lane, 1);
@@ -653,6 +691,8 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
         if (ok && elected) linear_commit<false>(accf);
         __syncwarp();
     } else {
+        LinearSplitEpilogue<NB> epilogue;
+        epilogue.fetch(p, rank, split, row0, col0, rows);
         // The sums of the rows that exist, to shared memory: 16 bytes apart beyond their length, so that the stores of eight threads
         // (eight rows) fall on all banks.  The ring is free: every copy has landed and every MMA has read it.
         ok = mbar_wait(accf, 0, abort_flag);
@@ -661,7 +701,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             linear_fence_after();
             float *red = reinterpret_cast<float *>(smem) + (size_t)(q * 32 + lane) * (NB + 4) + c0;
             const bool mine = q * 32 + lane < rows;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < NB / 2; c += 32) {
                 float z[32];
                 linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(c0 + c), z);
@@ -673,28 +713,30 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
             }
             linear_fence_before();
         }
+        if (!ok) settle_after_timeout();
+        __syncwarp();
+        linear_cluster_sync();       // all parts' sums are in their CTAs' shared memory
+        if (ok) {
+            const uint32_t sums = smem_u32(smem);
+            switch (split) {
+            case 1: epilogue.template finish<1>(p, sums, rank, row0, col0, rows); break;
+            case 2: epilogue.template finish<2>(p, sums, rank, row0, col0, rows); break;
+            case 3: epilogue.template finish<3>(p, sums, rank, row0, col0, rows); break;
+            case 4: epilogue.template finish<4>(p, sums, rank, row0, col0, rows); break;
+            case 5: epilogue.template finish<5>(p, sums, rank, row0, col0, rows); break;
+            case 6: epilogue.template finish<6>(p, sums, rank, row0, col0, rows); break;
+            case 7: epilogue.template finish<7>(p, sums, rank, row0, col0, rows); break;
+            default: epilogue.template finish<8>(p, sums, rank, row0, col0, rows); break;
+            }
+        }
     }
-    if (!ok) {
-        settle_after_timeout();
-        if (lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
+    if (warp >= LS_DRAIN_WARPS) {
+        if (!ok) settle_after_timeout();
+        __syncwarp();
+        linear_cluster_sync();       // (as the draining warps above)
     }
+    if (!ok && lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
     __syncwarp();
-    linear_cluster_sync();       // all parts' sums are in their CTAs' shared memory
-
-    uint32_t part_base[LS_MAX_SPLIT];
-#pragma unroll
-    for (int part = 0; part < LS_MAX_SPLIT; ++part)
-        part_base[part] = split == 1 ? smem_u32(smem) : linear_map_to_cta(smem_u32(smem), (uint32_t)min(part, split - 1));
-    switch (split) {
-    case 1: linear_split_finish<NB, 1>(p, part_base, rank, row0, col0, rows); break;
-    case 2: linear_split_finish<NB, 2>(p, part_base, rank, row0, col0, rows); break;
-    case 3: linear_split_finish<NB, 3>(p, part_base, rank, row0, col0, rows); break;
-    case 4: linear_split_finish<NB, 4>(p, part_base, rank, row0, col0, rows); break;
-    case 5: linear_split_finish<NB, 5>(p, part_base, rank, row0, col0, rows); break;
-    case 6: linear_split_finish<NB, 6>(p, part_base, rank, row0, col0, rows); break;
-    case 7: linear_split_finish<NB, 7>(p, part_base, rank, row0, col0, rows); break;
-    default: linear_split_finish<NB, 8>(p, part_base, rank, row0, col0, rows); break;
-    }
     linear_cluster_sync();       // (the others may still read this CTA's sums)
     if (warp == LS_DRAIN_WARPS + L_PRODUCERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB));
 }
