@@ -799,7 +799,7 @@ struct LinearChoice {
 
 // Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
 // shapes (M = 1 .. 2048; K and N from 512 to 11008; 16 and 8 bits, B 0.25 to 90 MB, three sets of operands in turn): what the rule picks takes
-// 1.0 % longer than the best variant on average, 14 % at most.  (What all variants have in common, about 3 us, is left out.)
+// 0.8 % longer than the best variant on average, 10 % at most.
 static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
 {
     LinearChoice c = {0, 0, 0, 128, 1};
@@ -808,12 +808,12 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
     double best = 1e30;
     // a K step: the MMAs, or the copies, which are slower the more SMs copy
     auto step = [&](int nb, long tiles) {
-        return std::max(nb * 0.00156, (256 + nb) * (0.000396 + 0.000246 * (double)std::min<long>(tiles, pairs) / pairs));
+        return std::max(nb * 0.00154, (256 + nb) * (0.000407 + 0.000204 * (double)std::min<long>(tiles, pairs) / pairs));
     };
     for (int nb = 64; nb <= 256; nb += 64) {
         const int across = ceil_div(N, nb);
         const long tiles = (long)down * across, rounds = (tiles + pairs - 1) / pairs;
-        const double fixed = 0.62 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm) + 0.62 * (rounds - 1);
+        const double fixed = 4.08 + 0.88 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm) + 3.0 * (rounds - 1);
         if (t < best) best = t, c.pair_nb = nb, c.columns = c.tail_nb = 0;
         // where the last round is partly filled: whole rounds of this width, the columns that are left in narrower tiles
         const int columns = (int)std::min<long>(across, tiles / pairs * pairs / down);
@@ -821,7 +821,7 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
         for (int tail = 64; tail < nb; tail += 64) {
             const long first = (long)columns * down, all = first + (long)ceil_div(N - columns * nb, tail) * down;
             const long wide = (first + pairs - 1) / pairs, narrow = (all + pairs - 1) / pairs - wide;
-            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 0.62 * (wide + narrow - 1);
+            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 3.0 * (wide + narrow - 1);
             if (tt < 0.98 * best) best = tt, c.pair_nb = nb, c.tail_nb = tail, c.columns = columns;
         }
     }
@@ -833,11 +833,11 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
             const long ctas = tiles * split, rounds = (ctas + 2 * sms - 1) / (2 * sms);
             const int steps = ceil_div(ksteps, split);
             const double kb = (box + nb) * (L_KBYTES / 1000.0);                // copied per step and CTA
-            const double one = rounds * steps * std::max(0.191, kb / 67.7), all = ctas * steps * kb / 15350.0;
+            const double one = rounds * steps * std::max(0.293, kb / 62.9), all = ctas * steps * kb / 14210.0;
             // (fewer CTAs than the SMs have room for have less of HBM under way)
-            const double bytes = hbm * (1.0 + 0.5 * (1.0 - (double)ctas / (rounds * 2 * sms)));
-            const double t = 0.58 + 0.82 * rows * nb / 16384 + std::max({one, all, bytes}) + 0.06 * (rounds - 1) + 0.93 * ctas / (2 * sms) +
-                             (split - 1) * (0.03 + (double)M * N * 4 / 3.32e6);   // sums through distributed shared memory
+            const double bytes = hbm * (1.0 + 0.94 * (1.0 - (double)ctas / (rounds * 2 * sms)));
+            const double t = 3.86 + 1.76 * rows * nb / 16384 + std::max({one, all, bytes}) + 1.57 * ctas / (2 * sms) +
+                             (split - 1) * (0.043 + (double)M * N * 4 / 4.4e6);   // sums through distributed shared memory
             if (t < best) best = t, c = {0, 0, 0, nb, split};
         }
     }
