@@ -162,6 +162,12 @@ __device__ __forceinline__ void linear_cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The same without ordering memory: for the barriers' set-up (fenced by itself) and the end of the kernel, where no data passes.
+__device__ __forceinline__ void linear_cluster_meet()
+{
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t linear_map_to_cta(uint32_t addr, uint32_t rank)
 {
     uint32_t r;
@@ -266,7 +272,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     }
     linear_fence_before();
     __syncthreads();
-    linear_cluster_sync();
+    linear_cluster_meet();
     linear_fence_after();
     grid_launch_dependents();
     grid_dependency_wait();
@@ -476,7 +482,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
     }
     linear_fence_before();
     __syncthreads();
-    linear_cluster_sync();        // nothing of the other CTA is touched after this
+    linear_cluster_meet();        // nothing of the other CTA is touched after this
     if (warp == L_PRODUCERS) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(LP_TMEM_COLS));
 }
 
@@ -737,7 +743,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
     }
     if (!ok && lane == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
     __syncwarp();
-    linear_cluster_sync();       // (the others may still read this CTA's sums)
+    linear_cluster_meet();       // (the others may still read this CTA's sums)
     if (warp == LS_DRAIN_WARPS + L_PRODUCERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB));
 }
 
@@ -797,23 +803,21 @@ struct LinearChoice {
     int nb, split;        // split kernel
 };
 
-// Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 176
-// shapes (M = 1 .. 2048; K and N from 512 to 11008; 16 and 8 bits, B 0.25 to 90 MB, three sets of operands in turn): what the rule picks takes
-// 0.8 % longer than the best variant on average, 10 % at most.
+// Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 216
+// shapes (M = 1 .. 4096; K and N from 64 to 11008; 16 and 8 bits, B up to 90 MB, three sets of operands in turn): what the rule picks takes
+// 0.6 % longer than the best variant on average, 11 % at most.
 static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
 {
     LinearChoice c = {0, 0, 0, 128, 1};
     const int pairs = std::max(1, sms / 2), down = ceil_div(M, 256);
-    const double hbm = ((double)M + N) * ksteps * L_KBYTES / 6.5e6;            // operands once
+    const double hbm = (((double)M + N) * ksteps * L_KBYTES + 2.0 * M * N) / 6.5e6;   // operands and C once
     double best = 1e30;
-    // a K step: the MMAs, or the copies, which are slower the more SMs copy
-    auto step = [&](int nb, long tiles) {
-        return std::max(nb * 0.00154, (256 + nb) * (0.000407 + 0.000204 * (double)std::min<long>(tiles, pairs) / pairs));
-    };
+    // a K step is as long as its copies take, which are slower the more SMs copy
+    auto step = [&](int nb, long tiles) { return (256 + nb) * (0.000562 + 0.000293 * (double)std::min<long>(tiles, pairs) / pairs); };
     for (int nb = 64; nb <= 256; nb += 64) {
         const int across = ceil_div(N, nb);
         const long tiles = (long)down * across, rounds = (tiles + pairs - 1) / pairs;
-        const double fixed = 4.08 + 0.88 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm) + 3.0 * (rounds - 1);
+        const double fixed = 5.68 + 0.73 * nb / 64, t = fixed + std::max(rounds * ksteps * step(nb, tiles), hbm) + 1.5 * (rounds - 1);
         if (t < best) best = t, c.pair_nb = nb, c.columns = c.tail_nb = 0;
         // where the last round is partly filled: whole rounds of this width, the columns that are left in narrower tiles
         const int columns = (int)std::min<long>(across, tiles / pairs * pairs / down);
@@ -821,23 +825,24 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
         for (int tail = 64; tail < nb; tail += 64) {
             const long first = (long)columns * down, all = first + (long)ceil_div(N - columns * nb, tail) * down;
             const long wide = (first + pairs - 1) / pairs, narrow = (all + pairs - 1) / pairs - wide;
-            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 3.0 * (wide + narrow - 1);
+            const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 1.5 * (wide + narrow - 1);
             if (tt < 0.98 * best) best = tt, c.pair_nb = nb, c.tail_nb = tail, c.columns = columns;
         }
     }
     const int rows = std::min(M, 128), box = ceil_div(rows, 8) * 8;
     for (int nb = 64; nb <= 128; nb += 64) {
         const long tiles = (long)ceil_div(M, 128) * ceil_div(N, nb);
+        const double drain = (double)rows * nb / 16384;
         for (int split : {1, 2, 3, 4, 6, 8}) {
             if (split > ksteps) break;
             const long ctas = tiles * split, rounds = (ctas + 2 * sms - 1) / (2 * sms);
             const int steps = ceil_div(ksteps, split);
             const double kb = (box + nb) * (L_KBYTES / 1000.0);                // copied per step and CTA
-            const double one = rounds * steps * std::max(0.293, kb / 62.9), all = ctas * steps * kb / 14210.0;
+            const double one = rounds * std::max(steps * std::max(0.412, kb / 52.5), 0.52 * drain), all = ctas * steps * kb / 11800.0;
             // (fewer CTAs than the SMs have room for have less of HBM under way)
-            const double bytes = hbm * (1.0 + 0.94 * (1.0 - (double)ctas / (rounds * 2 * sms)));
-            const double t = 3.86 + 1.76 * rows * nb / 16384 + std::max({one, all, bytes}) + 1.57 * ctas / (2 * sms) +
-                             (split - 1) * (0.043 + (double)M * N * 4 / 4.4e6);   // sums through distributed shared memory
+            const double bytes = hbm * (1.0 + 0.66 * (1.0 - (double)ctas / (rounds * 2 * sms)));
+            const double t = 3.42 + 5.2 * drain + std::max({one, all, bytes}) + 1.55 * ctas / (2 * sms) +
+                             (split - 1) * (0.128 + (double)M * N * 4 / 2.86e6);   // sums through distributed shared memory
             if (t < best) best = t, c = {0, 0, 0, nb, split};
         }
     }
