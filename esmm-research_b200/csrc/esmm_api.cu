@@ -308,7 +308,7 @@ const char *esmm_strerror(int status)
 }
 
 const char *esmm_last_cuda_error(void) { return esmm::g_cuda_error; }
-int esmm_version(void) { return 110; }
+int esmm_version(void) { return 120; }
 
 int esmm_tuning_set(const char *name, int value)
 {
