@@ -374,7 +374,7 @@ int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float 
  *   out_dtype   type of C, bias, residual and pre: dtype, or ESMM_F16 / ESMM_BF16 for e4m3 operands
  *   d_C         M x N, overwritten; not A or B
  *   d_a_scale   M floats or NULL (ones);  d_b_scale  N floats or NULL (ones)
- *   d_bias      N values or NULL;  d_residual  M x N or NULL, may be d_C;  d_pre  M x N or NULL (kept for the backward pass)
+ *   d_bias      N values or NULL;  d_residual  M x N or NULL, may be d_C;  d_pre  M x N or NULL (kept for the backward pass), not d_C
  * so a layer's gradients are calls of it: dA = dZ B^T (trans_b = 1 on the forward pass's B), dB = A^T dZ (trans_a = 1).
  * trans_a with trans_b, and e4m3 operands other than trans_a = 0, trans_b = 1, are ESMM_ERR_UNSUPPORTED.
  * N % 8 == 0; the stored rows of A and B are whole 16-byte vectors (K, M or N a multiple of 8, K of 16 for e4m3), else

@@ -265,3 +265,28 @@ def test_epilogue_backward(cuda, pkg, t, activation, m, n):
     pkg.epilogue_backward(m, n, d.code(pkg, t), dc.data_ptr(), pre.data_ptr(), d.act_code(pkg, activation), dc.data_ptr())
     pkg.device_status()
     assert torch.equal(alone, db[0]) and torch.equal(dc, dz)
+
+
+def test_outputs_past_32_bit_offsets(cuda, pkg):
+    """C, residual and gradients of more than 2^31 values: the last rows come out as they do by themselves."""
+    m, n, k = 270000, 8192, 64
+    a = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    a[-200:] = torch.randn((200, k), device="cuda").bfloat16()
+    b = torch.randn((k, n), device="cuda").bfloat16()
+    c = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    c[-200:] = torch.randn((200, n), device="cuda").bfloat16()
+    c[:-200] = 1.0
+    res, small = c[-200:].clone(), torch.empty((200, n), dtype=torch.bfloat16, device="cuda")
+    pkg.linear(m, n, k, pkg.BF16, a.data_ptr(), b.data_ptr(), pkg.BF16, c.data_ptr(), residual=c.data_ptr(), activation=pkg.ACT_SILU)
+    pkg.linear(200, n, k, pkg.BF16, a[-200:].data_ptr(), b.data_ptr(), pkg.BF16, small.data_ptr(), residual=res.data_ptr(), activation=pkg.ACT_SILU)
+    pkg.device_status()
+    # (k = 64 is one run of additions in either kernel)
+    assert torch.equal(c[-200:], small) and bool((c[:1000] == 1.0).all()) and bool((c[m // 2:m // 2 + 1000] == 1.0).all())
+    ws = torch.empty(pkg.epilogue_backward_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    db = torch.empty(n, dtype=torch.bfloat16, device="cuda")
+    pkg.epilogue_backward(m, n, pkg.BF16, c.data_ptr(), c.data_ptr(), pkg.ACT_RELU, c.data_ptr(), db.data_ptr(), ws.data_ptr())
+    pkg.epilogue_backward(200, n, pkg.BF16, small.data_ptr(), small.data_ptr(), pkg.ACT_RELU, small.data_ptr())
+    pkg.device_status()
+    assert torch.equal(c[-200:], small)
+    total = small.double().sum(0) + (m - 200)
+    d.assert_close(db, total, d.half_step("bf16") * total.abs() + 2.0 ** -20 * total.abs())

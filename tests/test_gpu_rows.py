@@ -319,3 +319,42 @@ def test_norms_on_two_streams_at_once(cuda, pkg):
     for r, e in zip(runs, want):
         for key, v in zip(("h", "out", "dx", "dw"), e):
             assert torch.equal(r[key], v)
+
+
+@pytest.mark.parametrize("m,k", [(40, 512), (40, 1501), (3, 12000), (2, 40000)])
+def test_norm_backward_over_its_inputs(cuda, pkg, m, k):
+    x, _, w, dout, dsum = tensors(m, k, "bf16", seed=8)
+    rstd = d.norm(x, None, w, EPS)[1].float()
+    want = torch.empty_like(x)
+    call = lambda g, s, to: pkg.rmsnorm_backward(m, k, pkg.BF16, g.data_ptr(), x.data_ptr(), w.data_ptr(), rstd.data_ptr(), s.data_ptr(), to.data_ptr())  # noqa: E731
+    call(dout, dsum, want)
+    over = dout.clone()
+    call(over, dsum, over)
+    call(dout, dsum, dsum)
+    pkg.device_status()
+    assert torch.equal(over, want) and torch.equal(dsum, want)
+
+
+def test_rows_past_32_bit_offsets(cuda, pkg):
+    """More than 2^31 elements: the last rows come out as they do by themselves."""
+    m, k = 70000, 32768
+    x = torch.empty((m, k), dtype=torch.bfloat16, device="cuda")
+    x.fill_(0.5)
+    x[-3:] = torch.randn((3, k), device="cuda").bfloat16()
+    out, rstd, scale = torch.empty_like(x), torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    pkg.rmsnorm(m, k, pkg.BF16, x.data_ptr(), 0, 0, EPS, 0, pkg.BF16, out.data_ptr(), 0, rstd.data_ptr())
+    small, r = torch.empty((3, k), dtype=torch.bfloat16, device="cuda"), torch.empty(3, device="cuda")
+    # (one or four vectors per thread: sums in another order, a step of the type at most)
+    pkg.rmsnorm(3, k, pkg.BF16, x[-3:].data_ptr(), 0, 0, EPS, 0, pkg.BF16, small.data_ptr(), 0, r.data_ptr())
+    pkg.device_status()
+    assert torch.allclose(rstd[-3:], r, rtol=1e-6) and bool((out[:5].float() == 1.0).all())
+    d.assert_close(out[-3:], small.double(), 2 * d.half_step("bf16") * small.double().abs() * 1.01)
+    dx, dsmall = out, torch.empty_like(small)                  # the gradient over its own input's buffer
+    dx[-3:] = small
+    pkg.rmsnorm_backward(m, k, pkg.BF16, dx.data_ptr(), x.data_ptr(), 0, rstd.data_ptr(), 0, dx.data_ptr())
+    pkg.rmsnorm_backward(3, k, pkg.BF16, small.data_ptr(), x[-3:].data_ptr(), 0, rstd[-3:].data_ptr(), 0, dsmall.data_ptr())
+    q, qs = torch.empty((m, k), dtype=torch.uint8, device="cuda"), torch.empty((3, k), dtype=torch.uint8, device="cuda")
+    pkg.quantize_rows(m, k, pkg.BF16, x.data_ptr(), q.data_ptr(), scale.data_ptr())
+    pkg.quantize_rows(3, k, pkg.BF16, x[-3:].data_ptr(), qs.data_ptr(), r.data_ptr())
+    pkg.device_status()
+    assert torch.equal(dx[-3:], dsmall) and torch.equal(q[-3:], qs) and torch.equal(scale[-3:], r)
