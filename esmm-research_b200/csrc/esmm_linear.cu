@@ -349,18 +349,20 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
         // ---------------- epilogue: a row per thread, 64 columns at a time through the warp's staging boxes ----------------
         const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns 64 (half + 2 c) ..
         const int tid = threadIdx.x - 128;
-        char *box = smem + p.box_off + w * p.boxes * LP_BOX;
+        char *boxes = smem + p.box_off + w * p.boxes * LP_BOX;
         float *col_scale = reinterpret_cast<float *>(smem + LP_COLUMN_OFF), *col_bias = col_scale + LP_MAX_NB;
         const uint32_t res_bar = res0 + 8 * w;
         const bool scaled = F8 || p.a_scale != nullptr || p.b_scale != nullptr;
         auto unpack2 = [](uint32_t v) { return BF16 ? unpack_bf16(v) : unpack_f16(v); };
         auto pack2 = [](float lo, float hi) { return BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi); };
-        // Until this warp's box for the next piece is free: with two boxes and one store per piece the last store may still be under way.
+        // The warp's boxes are taken in turn, whatever tile a piece is of.  Until the next one is free: with two boxes and one store per piece the
+        // last store, which reads the other box, may still be under way.
         auto box_free = [&]() {
             if (p.boxes == 2 && !p.has_pre) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         };
         uint32_t turn = 0, res_phase = 0;
+        int which = 0;                                            // the next piece's box
         // (after a wait that ran out these warps go on through all tiles, doing nothing, so that none is missing at their barrier; the waits return
         // at once then)
         for (int tile = pair; tile < p.num_tiles; tile += num_pairs, ++turn) {
@@ -371,7 +373,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
             const uint32_t ab = turn & 1u;
             auto fetch_residual = [&](int c) {
                 mbar_arrive_expect_tx(res_bar, (uint32_t)LP_BOX);
-                tma_load_2d(smem_u32(box) + (uint32_t)(c * (p.boxes - 1) * LP_BOX), &maps.residual, col0 + 128 * c, row0, res_bar);
+                tma_load_2d(smem_u32(boxes) + (uint32_t)(which * LP_BOX), &maps.residual, col0 + 128 * c, row0, res_bar);
             };
             if (lane == 0 && ok && p.has_residual && chunks > 0 && row0 < p.M && col0 < p.N) {
                 box_free();
@@ -399,7 +401,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 const int c = passes == 2 ? i >> 1 : i;
                 const bool pre_pass = passes == 2 && (i & 1);
                 const int col = col0 + 128 * c;
-                char *mine = box + c * (p.boxes - 1) * LP_BOX + lane * 128;
+                char *box = boxes + which * LP_BOX, *mine = box + lane * 128;
                 const bool inside = row0 < p.M && col < p.N;      // (a box wholly outside C is not stored; the rest is clipped)
                 const bool adds = p.has_residual && inside && !pre_pass;
                 float z[64];
@@ -407,7 +409,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 linear_tmem_ld(from, z);
                 linear_tmem_ld(from + 32, z + 32);
                 if (lane == 0) {
-                    if (!(p.has_residual && i == 0)) box_free();
+                    if (!(adds && i == 0)) box_free();            // (before the tile's first residual it was waited for)
                     if (adds && i) fetch_residual(c);
                 }
                 linear_tmem_wait(z);
@@ -469,10 +471,11 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 if (lane == 0) {
                     if (inside && ok)
                         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(pre_pass ? &maps.pre : &maps.c),
-                                     "r"(col), "r"(row0), "r"(smem_u32(box) + (uint32_t)(c * (p.boxes - 1) * LP_BOX))
+                                     "r"(col), "r"(row0), "r"(smem_u32(box))
                                      : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
+                if (passes == 1 || pre_pass) which ^= p.boxes - 1;
             }
             if (chunks == 0 && lane == 0)                         // (the other four warps do all of a narrow tile)
                 asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(linear_map_to_cta(acce0 + 8 * ab, 0)) : "memory");

@@ -113,6 +113,17 @@ def test_residual_in_place(cuda, pkg, tuning, pair):
     check(pkg, 300, 328, 128, "f16", bias=True, residual=True, inplace=True, activation="relu")
 
 
+@pytest.mark.parametrize("pair", [64, 128, 192, 256])
+@pytest.mark.parametrize("k", [64, 1088])
+def test_many_tiles_per_cta(cuda, pkg, tuning, pair, k):
+    """Short K (two staging boxes per warp) and long (one), one and two pieces per warp and tile, edges in the last tile row and column."""
+    tuning("LINEAR_PAIR", pair)
+    m, n = (2320, 2072) if pair < 256 else (2320, 4136)
+    for residual in (False, True):
+        for pre in (False, True):
+            check(pkg, m, n, k, "bf16", bias=True, residual=residual, pre=pre, activation="relu")
+
+
 def test_long_k_and_many_tiles(cuda, pkg):
     check(pkg, 16, 256, 16384, "bf16")
     check(pkg, 2100, 4104, 512, "bf16", bias=True, activation="silu", residual=True)
