@@ -11,7 +11,8 @@
 // Two kernels:
 //   esmm_linear_pair_kernel<F8, BF16> large products.  Persistent, a cluster of two CTAs per 256 x 64 .. 256 tile (cta_group::2 MMAs): each CTA
 //       fetches its 128 rows of A and half the columns of B into a ring, one thread of the even CTA issues the MMAs, eight
-//       epilogue warps per CTA drain one of two accumulators in tensor memory while the other is filled.
+//       epilogue warps per CTA drain one of two accumulators in tensor memory while the other is filled.  Where tiles of 288 .. 512 columns make
+//       one round of what would be a round and a bit, both accumulators belong to one tile (two MMAs a step side by side).
 //   esmm_linear_split_kernel<NB, F8>  few rows or few tiles: one CTA per 128 x NB tile and part of K, the parts of a tile being one
 //       cluster.  The CTAs add up their accumulators through distributed shared memory in a fixed order, each of them finishing a
 //       share of the tile's outputs: no workspace, no atomics, the same bits on every call.  Its cost is the operands' bytes: all
@@ -33,7 +34,7 @@ namespace esmm {
 
 // What depends on a tile's width
 struct LinearTile {
-    int nb, tiles_n;                     // columns of a tile, tiles across
+    int nb, width, tiles_n;              // columns of an MMA and of a tile, tiles across
     int b_boxes, b_box_cols, b_box_bytes;   // copies of B per stage (K-major: one), columns and bytes of one
     int stage_bytes;                     // pair kernel: bytes that a CTA copies per stage
     uint32_t b_desc_hi, b_lbo, b_step;   // B's descriptors: high word, leading byte offset in place, from one MMA to the next
@@ -44,7 +45,9 @@ struct LinearParams {
     int M, N, ksteps;                    // K in steps of 128 bytes
     int tiles_m, num_tiles;
     // pair kernel: the first `wide_tiles` tiles cover the columns before `wide_cols` in the first width, the rest the others in the second
+    // (joined: a tile is as wide as both together, the accumulators side by side, and there is one tile per pair)
     LinearTile kind[2];
+    int joined;
     int wide_tiles, wide_cols;
     int group_m;
     int a_boxes;                         // copies of A per stage
@@ -54,6 +57,7 @@ struct LinearParams {
     int a_stage_bytes;                   // split kernel: of A's part of a stage
     int slot_bytes;                      // pair kernel: from one ring slot to the next
     int boxes, box_off;                  // pair kernel: staging boxes per epilogue warp, the first one's place
+    int column_off;                      // pair kernel: place of the tile's scales and biases by column
     uint32_t a_lbo;                      // leading byte offset of A's descriptors, in place
     uint32_t a_step;                     // from one MMA to the next along K, in 16-byte units
     int bf16;                            // type of C, bias, residual and pre: bfloat16 or float16
@@ -223,6 +227,7 @@ constexpr int LP_COLUMN_OFF = 224 * 1024;
 constexpr int LP_BAR_OFF = LP_COLUMN_OFF + 2 * LP_MAX_NB * 4;
 constexpr int LP_SMEM = LP_BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
 constexpr int LP_TMEM_COLS = 2 * LP_MAX_NB;
+constexpr int LP_JOINED_OFF = LP_A_BYTES + LP_MAX_NB / 2 * L_KBYTES;   // joined tiles: place of the second MMA's columns of B in a slot
 static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
 
 // Tile `item` of the launch: its width, tile row and first column.
@@ -232,7 +237,7 @@ __device__ __forceinline__ const LinearTile &linear_tile(const LinearParams &p, 
     const LinearTile &t = p.kind[second];
     int tn;
     tile_coords(second ? item - p.wide_tiles : item, p.tiles_m, t.tiles_n, tm, tn, p.group_m);
-    col = (second ? p.wide_cols : 0) + tn * t.nb;
+    col = (second ? p.wide_cols : 0) + tn * t.width;
     return t;
 }
 
@@ -299,7 +304,13 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 if (leader && lane == 0) mbar_arrive_expect_tx(full0 + 8 * slot, 2u * (uint32_t)t.stage_bytes);
                 __syncwarp();
                 const uint32_t dst = smem_u32(smem) + (uint32_t)(slot * p.slot_bytes);
-                linear_load_step<true>(p, t, maps, &maps.b[second], lane, step, row_a, row_b, dst, dst + LP_A_BYTES, linear_map_to_cta(full0 + 8 * slot, 0));
+                const uint32_t bar = linear_map_to_cta(full0 + 8 * slot, 0);
+                linear_load_step<true>(p, t, maps, &maps.b[second], lane, step, row_a, row_b, dst, dst + LP_A_BYTES, bar);
+                if (p.joined && lane >= 8 && lane - 8 < p.kind[1].b_boxes) {
+                    const LinearTile &u = p.kind[1];
+                    const int i = lane - 8, k = step * p.k_elems, r = col + t.nb + (int)rank * (u.nb / 2) + u.b_box_cols * i;
+                    linear_load<true>(dst + (uint32_t)(LP_JOINED_OFF + u.b_box_bytes * i), &maps.b[1], p.b_k_major ? k : r, p.b_k_major ? r : k, bar);
+                }
                 slot += L_PRODUCERS;
                 if (slot >= p.stages) {
                     slot -= p.stages;
@@ -333,6 +344,9 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                     // (a wait costs time even where the data is there: ask for the next step's while this one's MMAs are issued)
                     landed = mbar_test_wait(full0 + 8 * nslot, nslot ? phase : phase ^ 1u);
                     linear_mma_step<true, F8>(p, t, d, at | p.a_lbo, (at + (LP_A_BYTES >> 4)) | t.b_lbo, step != 0, elected);
+                    if (p.joined)
+                        linear_mma_step<true, F8>(p, p.kind[1], d + (uint32_t)LP_MAX_NB, at | p.a_lbo, (at + (LP_JOINED_OFF >> 4)) | p.kind[1].b_lbo,
+                                                  step != 0, elected);
                     if (elected) linear_commit<true>(empty0 + 8 * slot);
                     landed = __all_sync(0xFFFFFFFFu, landed);
                     if (++slot == p.stages) {
@@ -350,7 +364,9 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
         const int w = warp - 4, q = w & 3, half = w >> 2;         // TMEM lanes 32 q .., columns 64 (half + 2 c) ..
         const int tid = threadIdx.x - 128;
         char *boxes = smem + p.box_off + w * p.boxes * LP_BOX;
-        float *col_scale = reinterpret_cast<float *>(smem + LP_COLUMN_OFF), *col_bias = col_scale + LP_MAX_NB;
+        typedef typename std::conditional<BF16, __nv_bfloat16, __half>::type out_t;
+        const int columns = p.joined ? 2 * LP_MAX_NB : LP_MAX_NB;
+        float *col_scale = reinterpret_cast<float *>(smem + p.column_off), *col_bias = col_scale + columns;
         const uint32_t res_bar = res0 + 8 * w;
         const bool scaled = F8 || p.a_scale != nullptr || p.b_scale != nullptr;
         auto unpack2 = [](uint32_t v) { return BF16 ? unpack_bf16(v) : unpack_f16(v); };
@@ -366,7 +382,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
             const LinearTile &t = linear_tile(p, tile, second, tm, col);
             col += half * 64 + 128 * c;
             const int row = tm * 256 + (int)rank * 128 + q * 32;
-            if (c >= (t.nb / 64 - half + 1) / 2 || row >= p.M || col >= p.N) return;
+            if (half * 64 + 128 * c + 64 > t.width || row >= p.M || col >= p.N) return;   // (not a narrow piece's, which has no box)
             mbar_arrive_expect_tx(res_bar, (uint32_t)LP_BOX);
             tma_load_2d(smem_u32(boxes) + (uint32_t)(to * LP_BOX), &maps.residual, col, row, res_bar);
         };
@@ -376,7 +392,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
         for (int tile = pair; tile < p.num_tiles; tile += num_pairs, ++turn) {
             int second, tm, tile_col;
             const LinearTile &t = linear_tile(p, tile, second, tm, tile_col);
-            const int chunks = (t.nb / 64 - half + 1) / 2;        // of the tile's 64-column pieces, every other one: none to two
+            const int chunks = ((t.width + 63) / 64 - half + 1) / 2;   // of the tile's 64-column pieces, every other one: none to four
             const int row0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tile_col + half * 64;
             const uint32_t ab = turn & 1u;
             if (lane == 0 && ok && p.has_residual && !ahead) {    // (one box: the first piece's, under the wait for the accumulator)
@@ -385,15 +401,23 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
             }
             // the tile's scales and biases, a column per epilogue thread, under the wait for the accumulator
             const float sa = p.a_scale && row0 + lane < p.M ? p.a_scale[row0 + lane] : 1.0f;
-            float scale = 1.0f, bias = 0.0f;
-            if (tid < t.nb && tile_col + tid < p.N) {
-                if (p.b_scale) scale = p.b_scale[tile_col + tid];
-                if (p.bias) bias = to_float<typename std::conditional<BF16, __nv_bfloat16, __half>::type>(
-                                static_cast<const typename std::conditional<BF16, __nv_bfloat16, __half>::type *>(p.bias)[tile_col + tid]);
+            float scale[2], bias[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = tid + i * LP_MAX_NB;
+                scale[i] = 1.0f, bias[i] = 0.0f;
+                if (c < t.width && tile_col + c < p.N) {
+                    if (p.b_scale) scale[i] = p.b_scale[tile_col + c];
+                    if (p.bias) bias[i] = to_float<out_t>(static_cast<const out_t *>(p.bias)[tile_col + c]);
+                }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");        // every epilogue warp is through with the tile before
-            col_scale[tid] = scale;
-            col_bias[tid] = bias;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (i * LP_MAX_NB < columns) {
+                    col_scale[tid + i * LP_MAX_NB] = scale[i];
+                    col_bias[tid + i * LP_MAX_NB] = bias[i];
+                }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(accf0 + 8 * ab, (turn >> 1) & 1u, abort_flag) && ok);
             linear_fence_after();
@@ -407,7 +431,8 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 const int col = col0 + 128 * c;
                 char *box = boxes + which * LP_BOX, *mine = box + lane * 128;
                 const bool inside = row0 < p.M && col < p.N;      // (a box wholly outside C is not stored; the rest is clipped)
-                const bool adds = p.has_residual && inside && !pre_pass;
+                const bool narrow = half * 64 + 128 * c + 64 > t.width;   // 32 columns, the last piece of some joined tiles
+                const bool adds = p.has_residual && inside && !pre_pass && !narrow;
                 float z[64];
                 const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + ab * (uint32_t)LP_MAX_NB + (uint32_t)(half * 64 + 128 * c);
                 linear_tmem_ld(from, z);
@@ -452,6 +477,26 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
 #pragma unroll
                         for (int j = 0; j < 64; ++j) z[j] = activate<decltype(tag)::value>(z[j]);
                     });
+                if (narrow) {                                     // 64 bytes of each row without a box, whose store would take the next tile's columns along
+                    const size_t at = (size_t)(row0 + lane) * p.N + col;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (row0 + lane >= p.M || col + 8 * j >= p.N || !bounds_ok(at + 8 * j + 8 <= (size_t)p.M * p.N, p.status, 65)) continue;   // checked build: site 65
+                        if (p.has_residual && !pre_pass) {
+                            const uint4 r = *reinterpret_cast<const uint4 *>(static_cast<const out_t *>(p.residual) + at + 8 * j);
+                            const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = unpack2(rw[e]);
+                                z[8 * j + 2 * e] += f.x;
+                                z[8 * j + 2 * e + 1] += f.y;
+                            }
+                        }
+                        *reinterpret_cast<uint4 *>(static_cast<out_t *>(pre_pass ? p.pre : p.C) + at + 8 * j) =
+                            make_uint4(pack2(z[8 * j], z[8 * j + 1]), pack2(z[8 * j + 2], z[8 * j + 3]), pack2(z[8 * j + 4], z[8 * j + 5]), pack2(z[8 * j + 6], z[8 * j + 7]));
+                    }
+                    continue;                                     // (nothing follows it: a joined tile is its pair's only one)
+                }
                 if (adds) {
                     ok = mbar_wait(res_bar, res_phase, abort_flag);
                     res_phase ^= 1u;
@@ -818,14 +863,14 @@ static int linear_map(CUtensorMap *map, int dtype, const void *base, long inner,
 
 struct LinearChoice {
     int pair_nb;          // 64, 128, 192, 256: the width of the pair kernel's tiles; 0: the split kernel
-    int tail_nb, columns; // pair kernel: from this tile column on, tiles of another width
+    int tail_nb, columns; // pair kernel: from this tile column on, tiles of another width; no columns: every tile is that much wider (joined)
     int nb, split;        // split kernel
 };
 
 // Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 216
 // shapes (M = 1 .. 4096; K and N from 64 to 11008; 16 and 8 bits, B up to 90 MB, three sets of operands in turn): what the rule picks takes
 // 0.6 % longer than the best variant on average, 11 % at most.
-static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
+static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, int sms)
 {
     LinearChoice c = {0, 0, 0, 128, 1};
     const int pairs = std::max(1, sms / 2), down = ceil_div(M, 256);
@@ -847,6 +892,20 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
             const double tt = fixed + std::max(ksteps * (wide * step(nb, pairs) + narrow * step(tail, pairs)), hbm) + 1.5 * (wide + narrow - 1);
             if (tt < 0.98 * best) best = tt, c.pair_nb = nb, c.tail_nb = tail, c.columns = columns;
         }
+    }
+    // One tile per pair, wider than an MMA: as many columns as a single round takes.  (Two accumulators have no room beside each other then, so
+    // there is no second round.)  The second MMA's columns of B come in 32s, of which a CTA has half; stored K x N in boxes of 32.  The ring is shorter
+    // and nothing runs beside the epilogue: steps and fixed part are taken longer than those above, fitted to 44 shapes where this is possible
+    // (us, best of the other widths / joined: 512 x 4096 x 11008 bf16 40.1 / 36.2, 256 x 4096 x 20480 bf16 43.0 / 38.4, 1536 x 11008 x 4096 e4m3 54.8 / 50.7,
+    // but 2304 x 1024 x 4096 e4m3, where 512 columns are needed, 15.0 / 16.2).
+    const int per_pair = b_k_major ? 32 : 64;
+    auto joined_fits = [&](int extra) { return (long)down * ceil_div(N, LP_MAX_NB + extra) <= pairs; };
+    for (int extra = per_pair; extra <= LP_MAX_NB && (long)down * ceil_div(N, LP_MAX_NB) > pairs; extra += per_pair) {
+        if (!joined_fits(extra)) continue;
+        const int nb = LP_MAX_NB + extra;
+        const double t = 6.68 + 0.73 * nb / 64 + std::max(1.2 * ksteps * step(nb, (long)down * ceil_div(N, nb)), hbm);
+        if (t < best) best = t, c.pair_nb = LP_MAX_NB, c.tail_nb = extra, c.columns = 0;
+        break;
     }
     const int rows = std::min(M, 128), box = ceil_div(rows, 8) * 8;
     for (int nb = 64; nb <= 128; nb += 64) {
@@ -870,6 +929,8 @@ static LinearChoice linear_choose(int M, int N, int ksteps, int sms)
     const int forced_tail = tuning_get("LINEAR_TAIL", 0);
     if (c.pair_nb && forced_tail > 0 && forced_tail < c.pair_nb && forced_tail % 64 == 0 && N > c.pair_nb)
         c.tail_nb = forced_tail, c.columns = (ceil_div(N, c.pair_nb) + 1) / 2;
+    if (forced > LP_MAX_NB && forced <= 2 * LP_MAX_NB && forced % per_pair == 0 && joined_fits(forced - LP_MAX_NB))
+        c.pair_nb = LP_MAX_NB, c.tail_nb = forced - LP_MAX_NB, c.columns = 0;
     const int forced_split = tuning_get("LINEAR_SPLIT", 0);
     if (forced_split >= 1 && forced_split <= LS_MAX_SPLIT) c.split = std::min(forced_split, ksteps);
     const int forced_nb = tuning_get("LINEAR_COLUMNS", 0);
@@ -931,7 +992,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     p.status = device_status_ptr();
     if (!p.status) return ESMM_ERR_CUDA;
 
-    const LinearChoice choice = linear_choose(M, N, p.ksteps, sms);
+    const LinearChoice choice = linear_choose(M, N, p.ksteps, trans_b != 0, sms);
     const int rows_a = 128;                                                 // rows of A per CTA
     // few rows: boxes of as many as there are (what the MMA reads past them is never looked at)
     int a_box_rows = rows_a;
@@ -944,6 +1005,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     for (int i = 0; i < (choice.tail_nb ? 2 : 1); ++i) {
         LinearTile &t = p.kind[i];
         t.nb = i ? choice.tail_nb : choice.pair_nb ? choice.pair_nb : choice.nb;
+        t.width = t.nb;
         const int cols = choice.pair_nb ? t.nb / 2 : t.nb;                  // columns of B per CTA
         // MN-major B in boxes of 64 columns, or of 32 with the 64-byte swizzle where a CTA's columns are no multiple of 64
         const bool wide = cols % 64 == 0;
@@ -969,9 +1031,14 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
         if (!st && d_pre) st = linear_map(&maps.pre, out_dtype, d_pre, N, M, 64, 32);
         if (st) return st;
         p.tiles_m = ceil_div(M, 256);
-        p.kind[0].tiles_n = choice.tail_nb ? choice.columns : ceil_div(N, choice.pair_nb);
-        p.wide_cols = p.kind[0].tiles_n * choice.pair_nb;
-        if (choice.tail_nb) p.kind[1].tiles_n = ceil_div(N - p.wide_cols, choice.tail_nb);
+        p.joined = choice.tail_nb && !choice.columns;
+        if (p.joined) {
+            p.kind[0].width += choice.tail_nb;
+            p.kind[0].stage_bytes += p.kind[1].stage_bytes - LP_A_BYTES;
+        }
+        p.kind[0].tiles_n = choice.columns ? choice.columns : ceil_div(N, p.kind[0].width);
+        p.wide_cols = p.kind[0].tiles_n * p.kind[0].width;
+        if (choice.columns) p.kind[1].tiles_n = ceil_div(N - p.wide_cols, choice.tail_nb);
         if ((long)p.tiles_m * (p.kind[0].tiles_n + p.kind[1].tiles_n) > 0x7FFFFFFFL) return ESMM_ERR_TOO_LARGE;
         p.wide_tiles = p.tiles_m * p.kind[0].tiles_n;
         p.num_tiles = p.wide_tiles + p.tiles_m * p.kind[1].tiles_n;
@@ -981,8 +1048,9 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
         // time counts, and the next piece's residual is under way in the second box.
         p.boxes = p.ksteps >= 16 ? 1 : 2;
         const int staging = LP_EPI_WARPS * p.boxes * LP_BOX;
-        p.stages = std::min(LP_MAX_STAGES, (LP_COLUMN_OFF - staging) / p.slot_bytes);
-        p.box_off = LP_COLUMN_OFF - staging;
+        p.column_off = p.joined ? LP_BAR_OFF - 2 * 2 * LP_MAX_NB * 4 : LP_COLUMN_OFF;
+        p.box_off = (p.column_off - staging) & ~1023;
+        p.stages = std::min(LP_MAX_STAGES, p.box_off / p.slot_bytes);
         auto go = [&](auto kernel) -> int {
             ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)LP_SMEM, stream, maps, p));
             return ESMM_OK;

@@ -88,6 +88,19 @@ def test_two_tile_widths(cuda, pkg, tuning, pair, tail):
     check(pkg, 9, pair + 8, 64, "f16", bias=True)
 
 
+@pytest.mark.parametrize("pair", [288, 320, 352, 384, 480, 512])
+@pytest.mark.parametrize("k", [200, 1088])
+def test_tiles_wider_than_an_instruction(cuda, pkg, tuning, pair, k):
+    """Two accumulators side by side, the last piece 32 or 64 columns wide; the last tile's columns end inside its first or second part."""
+    tuning("LINEAR_PAIR", pair)
+    for trans in ("nn", "nt", "tn"):
+        for n in (pair, 3 * pair - 40, 2 * pair + 104):
+            check(pkg, 520, n, k, "bf16", trans_a=trans == "tn", trans_b=trans == "nt", activation="silu", bias=True, residual=True, pre=True)
+    check(pkg, 300, 2 * pair + 8, -(-k // 16) * 16, "e4m3", out="f16", bias=True, residual=True, scales=True, activation="gelu")
+    check(pkg, 300, 2 * pair + 8, k, "f16", trans_b=True, bias=True, residual=True, inplace=True)
+    check(pkg, 9, 8, k, "bf16", trans_b=True)
+
+
 @pytest.mark.parametrize("split", [1, 2, 3, 8])
 @pytest.mark.parametrize("columns", [64, 128])
 def test_parts_of_k(cuda, pkg, tuning, split, columns):
