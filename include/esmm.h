@@ -307,6 +307,7 @@ int esmm_sgemm_joint_tf32x3(int M, const float *d_A, const esmm_tf32x3_b *b, flo
 /*
  * What a feed-forward layer does beside its joint-sparse products: the norm before it, products in 16 and 8 bits with
  * everything that follows them in their epilogue, and the gradients of both.  No counterpart in the reference.
+ * The first call of each of them on a device sets it up (kernel attributes, the status word): make it outside stream capture.
  * Matrices are dense row-major as everywhere; d_ pointers are device pointers of the element type that the call names:
  */
 typedef enum esmm_dtype {
@@ -379,8 +380,7 @@ int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float 
  * trans_a with trans_b, and e4m3 operands other than trans_a = 0, trans_b = 1, are ESMM_ERR_UNSUPPORTED.
  * N % 8 == 0; the stored rows of A and B are whole 16-byte vectors (K, M or N a multiple of 8, K of 16 for e4m3), else
  * ESMM_ERR_SHAPE.  Matrices, bias, residual and pre are 16-byte aligned.  Any M >= 1 otherwise: few rows, or few tiles of C, are
- * taken by a kernel that splits K over a thread-block cluster.  No workspace, no atomics: equal calls give equal bits.  The first call on a
- * device sets kernel attributes; make it outside stream capture.
+ * taken by a kernel that splits K over a thread-block cluster.  No workspace, no atomics: equal calls give equal bits.
  */
 int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int trans_a, const void *d_B, int trans_b, int out_dtype, void *d_C,
                 const float *d_a_scale, const float *d_b_scale, const void *d_bias, const void *d_residual, void *d_pre,
