@@ -64,6 +64,13 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi)
     return r;
 }
 
+__device__ __forceinline__ float e4m3_to_float(uint8_t code)
+{
+    uint32_t halves;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"((uint16_t)code));
+    return unpack_f16(halves).x;
+}
+
 __device__ __forceinline__ float e4m3_scale(float amax) { return __fdiv_rn(fmaxf(amax, E4M3_TINY), E4M3_MAX); }
 
 // y / scale from inv = 1 / scale, with the remainder's correction: as good as the division itself, so that values next to a border

@@ -66,6 +66,12 @@ struct LinearParams {
     const void *bias;
     const void *residual;                // split kernel
     void *pre, *C;                       // split kernel
+    // pair kernel, relu with the values before it kept: those nearer to zero than this share of their size are summed again (0: none), from A and B as
+    // they are stored, with the strides of their two indices
+    float border;
+    int K;
+    const void *A, *B;
+    size_t a_row, a_k, b_col, b_k;
     int *status;
 };
 
@@ -222,13 +228,159 @@ constexpr int LP_BOX = 4096;                      // staging box of an epilogue 
 constexpr int LP_MAX_STAGES = 8;
 constexpr int LP_MAX_NB = 256;
 constexpr int LP_A_BYTES = 128 * L_KBYTES;
-// shared memory: ring, staging boxes (one or two per epilogue warp) | the tile's scales and biases by column | barriers, flags
+// shared memory: ring, staging boxes (one or two per epilogue warp) | the tile's scales and biases by column | barriers, flags | lists of elements
 constexpr int LP_COLUMN_OFF = 224 * 1024;
 constexpr int LP_BAR_OFF = LP_COLUMN_OFF + 2 * LP_MAX_NB * 4;
-constexpr int LP_SMEM = LP_BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
+constexpr int LP_LIST = 12;                       // elements next to relu's border that an epilogue warp notes
+constexpr int LP_LIST_OFF = LP_BAR_OFF + (2 * LP_MAX_STAGES + 4 + LP_EPI_WARPS) * 8 + 16;
+constexpr int LP_SMEM = LP_LIST_OFF + LP_EPI_WARPS * LP_LIST * 8;
 constexpr int LP_TMEM_COLS = 2 * LP_MAX_NB;
 constexpr int LP_JOINED_OFF = LP_A_BYTES + LP_MAX_NB / 2 * L_KBYTES;   // joined tiles: place of the second MMA's columns of B in a slot
 static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
+
+// ---- relu's border -----------------------------------------------------------------------------------------------------------------
+// relu's slope jumps at zero, so where the values before it are kept for the backward pass the sign of a small one has to be the sum's and not the
+// accumulation's.  The tensor cores cut every addition to the accumulator's 24 bits.  Their error next to zero, in units of Z's
+// standard deviation: 16-bit operands rms 5.8e-10 K, largest of some 690 elements 1.9e-6, 8.2e-6, 2.3e-5 at K = 784, 4096, 11008 (an FP32 FMA sum of
+// cuBLAS: 1.1e-6, 3.7e-6, 6.2e-6); e4m3 rms up to 2.7e-11 K.  So an element below ten times the rms, two of 2^19 at K = 784, is summed again in 64 bits (of 8000
+// sums that cancel halfway the largest error was 5.5 times it, and the next line's estimate may be a third too small).
+// The standard deviation is taken as (row's norm) (column's norm) / (norm) over a 32 x 64 piece, so that a column of small weights is not all border; a sum
+// that is exactly zero counts where it is the only one of its row and of its column in the piece (others are sums of zeros, as of pruned blocks).
+// An epilogue warp notes such elements of its pieces, as they lie rounded in its staging box, and the CTA sums them when its tiles are through, all epilogue
+// warps with a part of K each.  us with the values kept, silu / relu: 520 x 776 x 1032 fp16 9.2 / 11.1 (13.8 where an element is found), 2048 x 4096 x 11008 131 / 211
+// (some 800 elements, a column of B being 4096 lines of memory); summed by the warp alone within the piece 418, by a kernel of its own 220, and 17.5 for the small one.
+constexpr float LB_SHARE = 6e-9f, LB_SHARE_F8 = 3e-10f;
+constexpr int LB_MOST = LP_LIST / 2;          // elements per piece: more are no coincidence, and a bound on the time
+constexpr int LB_ROWS = 8;                    // in fewer rows a column's size does not show: the row's is taken alone
+
+template <bool F8, bool BF16> struct LinearOperand { typedef __half type; };
+template <> struct LinearOperand<false, true> { typedef __nv_bfloat16 type; };
+template <bool BF16> struct LinearOperand<true, BF16> { typedef uint8_t type; };
+__device__ __forceinline__ float linear_to_float(uint8_t v) { return e4m3_to_float(v); }
+__device__ __forceinline__ float linear_to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float linear_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Sum of op(A)_row,k op(B)_k,col in 64 bits over k = first, first + step, ... of the warp's lanes, in every lane; the order is fixed.  (Loads past K are of the
+// last k, so that none waits for a branch: all of a round are under way together.)
+template <bool F8, bool BF16>
+__device__ __noinline__ double linear_sum64(const LinearParams &p, int row, int col, int first, int step)
+{
+    typedef typename LinearOperand<F8, BF16>::type operand_t;
+    constexpr int U = 16;
+    double sum = 0.0;
+    if (bounds_ok(row < p.M && col < p.N, p.status, 66)) {   // checked build: site 66
+        const operand_t *a = static_cast<const operand_t *>(p.A) + (size_t)row * p.a_row, *b = static_cast<const operand_t *>(p.B) + (size_t)col * p.b_col;
+        for (long k0 = first; k0 < p.K; k0 += (long)step * U) {
+            operand_t x[U], y[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t k = (size_t)min(k0 + (long)step * u, (long)p.K - 1);
+                x[u] = a[k * p.a_k];
+                y[u] = b[k * p.b_k];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum = fma(k0 + (long)step * u < p.K ? (double)linear_to_float(x[u]) : 0.0, (double)linear_to_float(y[u]), sum);
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    return sum;
+}
+
+// the value before the activation from its 64-bit sum, over the one that is there
+template <bool BF16>
+__device__ __forceinline__ void linear_put(const LinearParams &p, int2 at, double sum)
+{
+    typedef typename std::conditional<BF16, __nv_bfloat16, __half>::type out_t;
+    if (!bounds_ok(at.x < p.M && at.y < p.N, p.status, 66)) return;
+    if (p.a_scale) sum *= (double)p.a_scale[at.x];
+    if (p.b_scale) sum *= (double)p.b_scale[at.y];
+    if (p.bias) sum += (double)to_float<out_t>(static_cast<const out_t *>(p.bias)[at.y]);
+    static_cast<out_t *>(p.pre)[(size_t)at.x * p.N + at.y] = from_float<out_t>((float)sum);
+}
+
+// Notes the elements of a staged piece (a row per lane from row0 on, columns from col0 on) that lie below the border.  cb: the columns' biases; reach: the share of the norm
+// of this lane's row of sums.  The warp's whole list is summed first where it has no room for a piece's.  Returns how many the list holds.  (Little code: fetching
+// it is what its first call in an SM takes.  With the norms of all rows and columns unrolled 520 x 776 x 1032 took 12.3 us.)
+template <bool F8, bool BF16>
+__device__ __noinline__ int linear_note_border(const LinearParams &p, const char *box, const float *cb, int row0, int col0, float reach, int2 *list, int noted)
+{
+    constexpr unsigned all = 0xFFFFFFFFu;
+    typedef typename std::conditional<BF16, __nv_bfloat16, __half>::type out_t;
+    const int lane = threadIdx.x & 31;
+    const char *mine = box + lane * 128;
+    const int there = min(64, p.N - col0);
+    auto value = [&](int j) { return to_float<out_t>(*reinterpret_cast<const out_t *>(mine + (((j >> 3) ^ (lane & 7)) << 4) + 2 * (j & 7))); };
+    unsigned long long hit = 0, zero = 0;
+#pragma unroll 4
+    for (int j = 0; j < there; ++j) {
+        const float z = value(j);
+        hit |= (unsigned long long)(fabsf(z) < reach) << j;
+        zero |= (unsigned long long)(z == cb[j]) << j;
+    }
+    if (zero & (zero - 1)) hit &= ~zero;                         // not the only one of its row
+    float whole = reach * reach;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) whole += __shfl_xor_sync(all, whole, d);
+    const float inv = rsqrtf(whole) * p.border, alone = rsqrtf((float)there);
+    unsigned long long columns = (unsigned long long)__reduce_or_sync(all, (unsigned)hit) | (unsigned long long)__reduce_or_sync(all, (unsigned)(hit >> 32)) << 32;
+    int left = LB_MOST;
+    while (columns && left > 0) {
+        const int j = __ffsll((long long)columns) - 1;
+        columns &= columns - 1;
+        const float z = value(j), v = row0 + lane < p.M ? z - cb[j] : 0.0f;
+        float down = v * v;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) down += __shfl_xor_sync(all, down, d);
+        const bool single = __popc(__ballot_sync(all, reach > 0.0f && v == 0.0f)) == 1;   // (a row of zeros is no column's)
+        unsigned rows = __ballot_sync(all, (hit >> j & 1) && (v != 0.0f || single) && fabsf(z) < reach * (p.M - row0 < LB_ROWS ? alone : sqrtf(down) * inv));
+        if (rows && noted > LP_LIST - LB_MOST && left == LB_MOST) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the pieces are in place
+            __syncwarp();
+            for (int e = 0; e < noted; ++e) {
+                const double sum = linear_sum64<F8, BF16>(p, list[e].x, list[e].y, lane, 32);
+                if (lane == 0) linear_put<BF16>(p, list[e], sum);
+            }
+            __syncwarp();
+            noted = 0;
+        }
+        for (; rows && left > 0; rows &= rows - 1, --left, ++noted)
+            if (lane == 0) list[noted] = make_int2(row0 + __ffs((int)rows) - 1, col0 + j);
+    }
+    return noted;
+}
+
+// By all epilogue warps when the CTA's tiles are through: every warp a part of K of all elements that they have noted, then the parts in their order.  (The ring is
+// free then: the copies of these tiles have landed and been read.)
+template <bool F8, bool BF16>
+__device__ __noinline__ void linear_sum_border(const LinearParams &p, char *smem, int tid, int noted)
+{
+    constexpr int ENTRIES = LP_EPI_WARPS * LP_LIST;
+    const int lane = tid & 31, w = tid >> 5;
+    int2 *lists = reinterpret_cast<int2 *>(smem + LP_LIST_OFF);
+    double *parts = reinterpret_cast<double *>(smem);
+    if (lane < LP_LIST && lane >= noted) lists[w * LP_LIST + lane].x = -1;
+    unsigned any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(any) : "r"(noted) : "memory");
+    if (!any) return;
+#pragma unroll 1
+    for (int e0 = 0; e0 < ENTRIES; e0 += 32) {
+        unsigned there = __ballot_sync(0xFFFFFFFFu, lists[e0 + lane].x >= 0);
+        for (; there; there &= there - 1) {
+            const int e = e0 + __ffs((int)there) - 1;
+            const double sum = linear_sum64<F8, BF16>(p, lists[e].x, lists[e].y, tid, 32 * LP_EPI_WARPS);
+            if (lane == 0) parts[e * LP_EPI_WARPS + w] = sum;
+        }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the pieces are in place
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (tid < ENTRIES && lists[tid].x >= 0) {
+        double sum = 0.0;
+        for (int i = 0; i < LP_EPI_WARPS; ++i) sum += parts[tid * LP_EPI_WARPS + i];
+        linear_put<BF16>(p, lists[tid], sum);
+    }
+}
+static_assert(LP_EPI_WARPS * LP_LIST % 32 == 0, "lists are looked through 32 elements at a time");
 
 // Tile `item` of the launch: its width, tile row and first column.
 __device__ __forceinline__ const LinearTile &linear_tile(const LinearParams &p, int item, int &second, int &tm, int &col)
@@ -374,6 +526,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
         // The warp's boxes are taken in turn, whatever tile a piece is of.  With two, the residual of the piece after the current one is fetched as
         // soon as the current one's has been read, into the other box (4096 x 512 x 4096 25.0 -> 23.9 us); with one, when its turn comes.
         const bool ahead = p.boxes == 2;
+        int noted = 0;                                            // elements next to relu's border in this warp's list
         uint32_t turn = 0, res_phase = 0;
         int which = 0;                                            // the current piece's box
         // (lane 0) residual of piece c of a tile to a box, if any of it lies inside C
@@ -462,6 +615,16 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                         z[j + 3] = z[j + 3] * sa * s4.w;
                     }
                 }
+                // whether an element of this row may lie below relu's border: none does that is not below the row's norm times the share, a column's norm being at
+                // most the piece's
+                const bool borders = pre_pass && p.border > 0.0f;
+                float reach = 0.0f;
+                if (borders) {
+                    float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) squares[j & 3] = fmaf(z[j], z[j], squares[j & 3]);
+                    reach = p.border * sqrtf((squares[0] + squares[1]) + (squares[2] + squares[3]));
+                }
                 if (p.bias) {
 #pragma unroll
                     for (int j = 0; j < 64; j += 4) {
@@ -470,6 +633,16 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                         z[j + 1] += b4.y;
                         z[j + 2] += b4.z;
                         z[j + 3] += b4.w;
+                    }
+                }
+                bool near = false;
+                if (borders) {
+#pragma unroll
+                    for (int j = 0; j < 64; j += 8) {
+                        float least = fabsf(z[j]);
+#pragma unroll
+                        for (int e = 1; e < 8; ++e) least = fminf(least, fabsf(z[j + e]));
+                        near = near || (col + j < p.N && least < reach);
                     }
                 }
                 if (p.activation && !pre_pass)
@@ -532,12 +705,15 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                                      : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
+                if (__any_sync(0xFFFFFFFFu, near))
+                    noted = linear_note_border<F8, BF16>(p, box, cb, row0, col, reach, reinterpret_cast<int2 *>(smem + LP_LIST_OFF) + w * LP_LIST, noted);
                 if (passes == 1 || pre_pass) which ^= p.boxes - 1;
             }
             if (chunks == 0 && lane == 0)                         // (the other four warps do all of a narrow tile)
                 asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(linear_map_to_cta(acce0 + 8 * ab, 0)) : "memory");
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // (what is written is there when the kernel has ended)
+        if (p.border > 0.0f) linear_sum_border<F8, BF16>(p, smem, tid, ok ? noted : 0);
     }
 
     if (!ok) {
@@ -867,10 +1043,11 @@ struct LinearChoice {
     int nb, split;        // split kernel
 };
 
+// `border`: elements next to relu's border are to be found, which the pair kernel does in the staging boxes of its pieces (of joined tiles the last has none).
 // Which kernel, tile widths and parts of K: the smallest estimated time in us.  The constants are fitted to the times of all variants on 216
 // shapes (M = 1 .. 4096; K and N from 64 to 11008; 16 and 8 bits, B up to 90 MB, three sets of operands in turn): what the rule picks takes
 // 0.6 % longer than the best variant on average, 11 % at most; on 663 shapes with their weights mostly in L2 1.5 %, 23 % at most.
-static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, int sms)
+static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, bool border, int sms)
 {
     LinearChoice c = {0, 0, 0, 128, 1};
     const int pairs = std::max(1, sms / 2), down = ceil_div(M, 256);
@@ -900,7 +1077,7 @@ static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, int 
     // but 2304 x 1024 x 4096 e4m3, where 512 columns are needed, 15.0 / 16.2).
     const int per_pair = b_k_major ? 32 : 64;
     auto joined_fits = [&](int extra) { return (long)down * ceil_div(N, LP_MAX_NB + extra) <= pairs; };
-    for (int extra = per_pair; extra <= LP_MAX_NB && (long)down * ceil_div(N, LP_MAX_NB) > pairs; extra += per_pair) {
+    for (int extra = per_pair; !border && extra <= LP_MAX_NB && (long)down * ceil_div(N, LP_MAX_NB) > pairs; extra += per_pair) {
         if (!joined_fits(extra)) continue;
         const int nb = LP_MAX_NB + extra;
         const double t = 6.68 + 0.73 * nb / 64 + std::max(1.2 * ksteps * step(nb, (long)down * ceil_div(N, nb)), hbm);
@@ -908,7 +1085,7 @@ static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, int 
         break;
     }
     const int rows = std::min(M, 128), box = ceil_div(rows, 8) * 8;
-    for (int nb = 64; nb <= 128; nb += 64) {
+    for (int nb = 64; nb <= 128 && !border; nb += 64) {
         const long tiles = (long)ceil_div(M, 128) * ceil_div(N, nb);
         const double drain = (double)rows * nb / 16384;
         for (int split : {1, 2, 3, 4, 6, 8}) {
@@ -925,11 +1102,11 @@ static LinearChoice linear_choose(int M, int N, int ksteps, bool b_k_major, int 
         }
     }
     const int forced = tuning_get("LINEAR_PAIR", -1);
-    if (forced == 0 || forced == 64 || forced == 128 || forced == 192 || forced == 256) c.pair_nb = forced, c.columns = c.tail_nb = 0;
+    if ((forced == 0 && !border) || forced == 64 || forced == 128 || forced == 192 || forced == 256) c.pair_nb = forced, c.columns = c.tail_nb = 0;
     const int forced_tail = tuning_get("LINEAR_TAIL", 0);
     if (c.pair_nb && forced_tail > 0 && forced_tail < c.pair_nb && forced_tail % 64 == 0 && N > c.pair_nb)
         c.tail_nb = forced_tail, c.columns = (ceil_div(N, c.pair_nb) + 1) / 2;
-    if (forced > LP_MAX_NB && forced <= 2 * LP_MAX_NB && forced % per_pair == 0 && joined_fits(forced - LP_MAX_NB))
+    if (!border && forced > LP_MAX_NB && forced <= 2 * LP_MAX_NB && forced % per_pair == 0 && joined_fits(forced - LP_MAX_NB))
         c.pair_nb = LP_MAX_NB, c.tail_nb = forced - LP_MAX_NB, c.columns = 0;
     const int forced_split = tuning_get("LINEAR_SPLIT", 0);
     if (forced_split >= 1 && forced_split <= LS_MAX_SPLIT) c.split = std::min(forced_split, ksteps);
@@ -992,7 +1169,18 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
     p.status = device_status_ptr();
     if (!p.status) return ESMM_ERR_CUDA;
 
-    const LinearChoice choice = linear_choose(M, N, p.ksteps, trans_b != 0, sms);
+    const bool border = d_pre && activation == ESMM_ACT_RELU;
+    if (border) {
+        p.border = (float)K * (f8 ? LB_SHARE_F8 : LB_SHARE);
+        p.K = K;
+        p.A = d_A;
+        p.B = d_B;
+        p.a_row = trans_a ? 1 : K;
+        p.a_k = trans_a ? M : 1;
+        p.b_col = trans_b ? K : 1;
+        p.b_k = trans_b ? 1 : N;
+    }
+    const LinearChoice choice = linear_choose(M, N, p.ksteps, trans_b != 0, border, sms);
     const int rows_a = 128;                                                 // rows of A per CTA
     // few rows: boxes of as many as there are (what the MMA reads past them is never looked at)
     int a_box_rows = rows_a;

@@ -377,6 +377,8 @@ int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float 
  *   d_a_scale   M floats or NULL (ones);  d_b_scale  N floats or NULL (ones)
  *   d_bias      N values or NULL;  d_residual  M x N or NULL, may be d_C;  d_pre  M x N or NULL (kept for the backward pass), not d_C
  * so a layer's gradients are calls of it: dA = dZ B^T (trans_b = 1 on the forward pass's B), dB = A^T dZ (trans_a = 1).
+ * With ESMM_ACT_RELU and d_pre, elements of pre next to zero are summed in 64 bits before their rounding: relu's slope jumps there, and its side is
+ * that of the sums, not of the accumulation's own error.
  * trans_a with trans_b, and e4m3 operands other than trans_a = 0, trans_b = 1, are ESMM_ERR_UNSUPPORTED.
  * N % 8 == 0; the stored rows of A and B are whole 16-byte vectors (K, M or N a multiple of 8, K of 16 for e4m3), else
  * ESMM_ERR_SHAPE.  Matrices, bias, residual and pre are 16-byte aligned.  Any M >= 1 otherwise: few rows, or few tiles of C, are

@@ -262,6 +262,100 @@ def test_gradients_against_differences(cuda, pkg):
         assert abs(got - slope) <= 2.0 ** -8 * (2 * mag + (spread * v.abs()).sum()), (key, got, slope)
 
 
+def planted(t, trans, m, n, half, seed):
+    """Operands in whose sums, at row 5 of every 32 and column 37 of every 64, the first half cancels the second and a small product of known sign is left over:
+    (A and B as stored, both in 64 bits, rows, columns)."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    k = 2 * half + 16
+    a = torch.randn((m, k), generator=gen, device="cuda")
+    b = torch.randn((k, n), generator=gen, device="cuda") * (1.0 if t == "e4m3" else k ** -0.5)
+    if t == "e4m3":
+        a, b = a * 16, b * 16
+    a, b = a.to(d.TYPES[t]).float(), b.to(d.TYPES[t]).float()
+    rows, cols = torch.arange(5, m, 32, device="cuda"), torch.arange(37, n, 64, device="cuda")
+    a[rows, half:2 * half] = -a[rows, :half]
+    b[half:2 * half, cols] = b[:half, cols]
+    a[rows, 2 * half:] = 0.0
+    b[2 * half:, cols] = 0.0
+    # 2^-22 of values of size one: above fp16's smallest steps, below the tensor cores' error of such a sum (e4m3: 2^-10 of a sum of about 2^13)
+    sign = torch.where(torch.rand((rows.numel(),), generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    a[rows, 2 * half] = sign * (2.0 ** -5 if t == "e4m3" else 2.0 ** -11)
+    b[2 * half, cols] = 2.0 ** -5 if t == "e4m3" else 2.0 ** -11
+    a, b = a.to(d.TYPES[t]), b.to(d.TYPES[t])
+    return (a.t().contiguous() if trans == "tn" else a, b.t().contiguous() if trans == "nt" else b, a.double(), b.double(), rows, cols)
+
+
+@pytest.mark.parametrize("t,trans,half", [("f16", "nn", 512), ("f16", "nt", 2048), ("f16", "tn", 392), ("bf16", "nn", 2048), ("bf16", "tn", 512), ("bf16", "nt", 5000),
+                                          ("e4m3", "nt", 2056)])
+@pytest.mark.parametrize("m,n,bias", [(520, 264, False), (296, 1032, True), (8, 136, False)])
+def test_relu_keeps_the_sign_of_sums_next_to_zero(cuda, pkg, t, trans, half, m, n, bias):
+    """relu's slope is that of the sums as they are, not as the accumulation's cuts leave them: pre at the planted places is the 64-bit sum, rounded once, and
+    dZ follows it."""
+    out = "bf16" if t == "e4m3" else t
+    ot = d.TYPES[out]
+    a, b, a64, b64, rows, cols = planted(t, trans, m, n, half, half)
+    k = a64.shape[1]
+    bias_t = torch.randn(n, device="cuda").to(ot) if bias else None
+    if bias:
+        bias_t[cols] = 0
+    sa = torch.rand(m, device="cuda") + 0.5 if t == "e4m3" else None
+    c, p, dz = (torch.empty((m, n), dtype=ot, device="cuda") for _ in range(3))
+    dc = torch.randn((m, n), device="cuda").to(ot)
+    pkg.linear(m, n, k, d.code(pkg, t), a.data_ptr(), b.data_ptr(), d.code(pkg, out), c.data_ptr(), trans_a=int(trans == "tn"), trans_b=int(trans == "nt"),
+               a_scale=0 if sa is None else sa.data_ptr(), bias=bias_t.data_ptr() if bias else 0, pre=p.data_ptr(), activation=pkg.ACT_RELU)
+    pkg.epilogue_backward(m, n, d.code(pkg, out), dc.data_ptr(), p.data_ptr(), pkg.ACT_RELU, dz.data_ptr())
+    pkg.device_status()
+    z, want, mag = d.linear(a64, b64, sa, None, bias_t, "relu", None)
+    off, u = d.sum_error(mag, k), d.half_step(out)
+    d.assert_close(p, z, off + u * (z.abs() + off) + d.smallest(out), "pre")
+    d.assert_close(c, want, off + u * (want.abs() + off) + d.smallest(out), "C")
+    at = (rows[:, None], cols[None, :])
+    assert bool((z[at] != 0).all())
+    d.assert_close(p[at], z[at], u * 1.01 * z[at].abs() + d.smallest(out), "planted")
+    assert torch.equal(dz[at], torch.where(z[at] > 0, dc[at], torch.zeros_like(dc[at])))
+
+
+def test_relu_border_of_many_tiles(cuda, pkg, tuning):
+    """More elements next to the border than a warp keeps until its tiles are through."""
+    tuning("LINEAR_PAIR", 64)
+    m, n = 8000, 2048
+    a, b, a64, b64, rows, cols = planted("f16", "nn", m, n, 264, 1)
+    k = a64.shape[1]
+    c, p = (torch.empty((m, n), dtype=torch.float16, device="cuda") for _ in range(2))
+    pkg.linear(m, n, k, pkg.F16, a.data_ptr(), b.data_ptr(), pkg.F16, c.data_ptr(), pre=p.data_ptr(), activation=pkg.ACT_RELU)
+    pkg.device_status()
+    z, _, mag = d.linear(a64, b64)
+    off, u, at = d.sum_error(mag, k), d.half_step("f16"), (rows[:, None], cols[None, :])
+    d.assert_close(p, z, off + u * (z.abs() + off) + d.smallest("f16"), "pre")
+    d.assert_close(p[at], z[at], u * 1.01 * z[at].abs() + d.smallest("f16"), "planted")
+
+
+def test_relu_border_is_not_where_columns_are_small_or_empty(cuda, pkg):
+    """Columns of tiny weights, of zeros, rows of zeros and of infinities beside ordinary ones: values as elsewhere, equal calls equal bits."""
+    m, n, k = 300, 520, 776
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    a = torch.randn((m, k), generator=gen, device="cuda").bfloat16()
+    b = (torch.randn((k, n), generator=gen, device="cuda") / k ** 0.5).bfloat16()
+    b[:, 3::8] *= 2.0 ** -30
+    b[:, 5::8] = 0
+    a[7], a[40:80] = 0, 0
+    a[9, 11] = float("inf")
+    got = []
+    for _ in range(2):
+        c, p = (torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        pkg.linear(m, n, k, pkg.BF16, a.data_ptr(), b.data_ptr(), pkg.BF16, c.data_ptr(), pre=p.data_ptr(), activation=pkg.ACT_RELU)
+        pkg.device_status()
+        got.append((c, p))
+    rest = torch.arange(m, device="cuda") != 9
+    z, want, mag = d.linear(a.double()[rest], b.double(), activation="relu")
+    off, u = d.sum_error(mag, k), d.half_step("bf16")
+    for c, p in got:
+        d.assert_close(p[rest], z, off + u * (z.abs() + off), "pre")
+        d.assert_close(c[rest], want, off + u * (want.abs() + off), "C")
+        assert torch.equal(torch.isfinite(p[9]), torch.isfinite(a[9].double() @ b.double()))
+    assert torch.equal(got[0][1].view(torch.int16), got[1][1].view(torch.int16))
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("activation", d.ACTS)
 @pytest.mark.parametrize("m,n", [(1, 8), (9, 264), (1001, 520), (4100, 72)])
