@@ -9,7 +9,7 @@
 // its gradients (dA = dZ B^T, dB = A^T dZ) need a transposed copy of anything.
 //
 // Two kernels:
-//   esmm_linear_pair_kernel<F8, BF16> large products.  Persistent, a cluster of two CTAs per 256 x 64 .. 256 tile (cta_group::2 MMAs): each CTA
+//   esmm_linear_pair_kernel           large products.  Persistent, a cluster of two CTAs per 256 x 64 .. 256 tile (cta_group::2 MMAs): each CTA
 //       fetches its 128 rows of A and half the columns of B into a ring, one thread of the even CTA issues the MMAs, eight
 //       epilogue warps per CTA drain one of two accumulators in tensor memory while the other is filled.  Where tiles of 288 .. 512 columns make
 //       one round of what would be a round and a bit, both accumulators belong to one tile (two MMAs a step side by side).
@@ -66,7 +66,7 @@ struct LinearParams {
     const void *bias;
     const void *residual;                // split kernel
     void *pre, *C;                       // split kernel
-    // pair kernel, relu with the values before it kept: those nearer to zero than this share of their size are summed again (0: none), from A and B as
+    // pair kernel, relu with the values before it kept: those nearer to zero than this share of their size are summed again, from A and B as
     // they are stored, with the strides of their two indices
     float border;
     int K;
@@ -316,7 +316,7 @@ __device__ __noinline__ int linear_note_border(const LinearParams &p, const char
     for (int j = 0; j < there; ++j) {
         const float z = value(j);
         hit |= (unsigned long long)(fabsf(z) < reach) << j;
-        zero |= (unsigned long long)(z == cb[j]) << j;
+        zero |= (unsigned long long)(fabsf(z) < reach && z == cb[j]) << j;   // (only there: beside a bias of size one many a sum is lost in the rounding)
     }
     if (zero & (zero - 1)) hit &= ~zero;                         // not the only one of its row
     float whole = reach * reach;
@@ -332,7 +332,7 @@ __device__ __noinline__ int linear_note_border(const LinearParams &p, const char
         float down = v * v;
 #pragma unroll
         for (int d = 16; d; d >>= 1) down += __shfl_xor_sync(all, down, d);
-        const bool single = __popc(__ballot_sync(all, reach > 0.0f && v == 0.0f)) == 1;   // (a row of zeros is no column's)
+        const bool single = __popc(__ballot_sync(all, zero >> j & 1)) == 1;
         unsigned rows = __ballot_sync(all, (hit >> j & 1) && (v != 0.0f || single) && fabsf(z) < reach * (p.M - row0 < LB_ROWS ? alone : sqrtf(down) * inv));
         if (rows && noted > LP_LIST - LB_MOST && left == LB_MOST) {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the pieces are in place
@@ -393,7 +393,8 @@ __device__ __forceinline__ const LinearTile &linear_tile(const LinearParams &p, 
     return t;
 }
 
-template <bool F8, bool BF16>
+// BORDER: with relu's border, apart from the others because its code in the epilogue costs them registers (2048 x 2048 x 4096 of bf16 27.6 us instead of 29.2).
+template <bool F8, bool BF16, bool BORDER>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LP_THREADS, 1)
 esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p)
 {
@@ -617,7 +618,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 }
                 // whether an element of this row may lie below relu's border: none does that is not below the row's norm times the share, a column's norm being at
                 // most the piece's
-                const bool borders = pre_pass && p.border > 0.0f;
+                const bool borders = BORDER && pre_pass;
                 float reach = 0.0f;
                 if (borders) {
                     float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -705,7 +706,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                                      : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
-                if (__any_sync(0xFFFFFFFFu, near))
+                if (BORDER && __any_sync(0xFFFFFFFFu, near))
                     noted = linear_note_border<F8, BF16>(p, box, cb, row0, col, reach, reinterpret_cast<int2 *>(smem + LP_LIST_OFF) + w * LP_LIST, noted);
                 if (passes == 1 || pre_pass) which ^= p.boxes - 1;
             }
@@ -713,7 +714,7 @@ esmm_linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_co
                 asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(linear_map_to_cta(acce0 + 8 * ab, 0)) : "memory");
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // (what is written is there when the kernel has ended)
-        if (p.border > 0.0f) linear_sum_border<F8, BF16>(p, smem, tid, ok ? noted : 0);
+        if (BORDER) linear_sum_border<F8, BF16>(p, smem, tid, ok ? noted : 0);
     }
 
     if (!ok) {
@@ -999,10 +1000,14 @@ static int linear_prepare(int dev, int *sms)
         int n = 0;
         ESMM_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         auto allow = [](auto kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); };
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, false>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, true>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, false>, SMEM_LIMIT));
-        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, false, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, false, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, true, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<false, true, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, false, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, false, true>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, true, false>, SMEM_LIMIT));
+        ESMM_CUDA_TRY(allow(esmm_linear_pair_kernel<true, true, true>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, false>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<64, true>, SMEM_LIMIT));
         ESMM_CUDA_TRY(allow(esmm_linear_split_kernel<128, false>, SMEM_LIMIT));
@@ -1243,8 +1248,12 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
             ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)(2 * pairs)), dim3(LP_THREADS), (size_t)LP_SMEM, stream, maps, p));
             return ESMM_OK;
         };
-        if (p.bf16) return f8 ? go(esmm_linear_pair_kernel<true, true>) : go(esmm_linear_pair_kernel<false, true>);
-        return f8 ? go(esmm_linear_pair_kernel<true, false>) : go(esmm_linear_pair_kernel<false, false>);
+        auto by_type = [&](auto with_border) -> int {
+            constexpr bool BORDER = decltype(with_border)::value;
+            if (p.bf16) return f8 ? go(esmm_linear_pair_kernel<true, true, BORDER>) : go(esmm_linear_pair_kernel<false, true, BORDER>);
+            return f8 ? go(esmm_linear_pair_kernel<true, false, BORDER>) : go(esmm_linear_pair_kernel<false, false, BORDER>);
+        };
+        return border ? by_type(std::true_type()) : by_type(std::false_type());
     }
 
     p.tiles_m = ceil_div(M, 128);

@@ -315,6 +315,21 @@ def test_relu_keeps_the_sign_of_sums_next_to_zero(cuda, pkg, t, trans, half, m, 
     assert torch.equal(dz[at], torch.where(z[at] > 0, dc[at], torch.zeros_like(dc[at])))
 
 
+def test_relu_border_beside_biases(cuda, pkg):
+    """Sums that a bias of size one swallows are not the zeros of pruned blocks: elements next to zero in their rows and columns keep their side."""
+    m, n = 296, 1032
+    a, b, a64, b64, rows, cols = planted("f16", "nn", m, n, 512, 512)
+    k, at = a64.shape[1], (rows[:, None], cols[None, :])
+    sums = a64 @ b64
+    for seed in range(20):
+        bias = torch.randn(n, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").half()
+        bias[cols] = 0
+        c, p = (torch.empty((m, n), dtype=torch.float16, device="cuda") for _ in range(2))
+        pkg.linear(m, n, k, pkg.F16, a.data_ptr(), b.data_ptr(), pkg.F16, c.data_ptr(), bias=bias.data_ptr(), pre=p.data_ptr(), activation=pkg.ACT_RELU)
+        pkg.device_status()
+        assert torch.equal(p[at] > 0, sums[at] > 0), seed
+
+
 def test_relu_border_of_many_tiles(cuda, pkg, tuning):
     """More elements next to the border than a warp keeps until its tiles are through."""
     tuning("LINEAR_PAIR", 64)
