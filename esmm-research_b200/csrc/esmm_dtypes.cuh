@@ -87,13 +87,41 @@ __device__ __forceinline__ float e4m3_quotient(float y, float scale, float inv)
 // exponential and one division, and no cancellation where tanh u is near -1.
 constexpr float GELU_U = 0.7978845608f, GELU_CUBE = 0.044715f;
 
+// gelu(z) = z Phi(z) = max(z, 0) - t Q(t) with t = |z| and the normal distribution's upper tail Q = 1 - Phi, so that no digit of a negative z's value cancels (from
+// 1 + erf(z / sqrt 2) it was 4 % off at z = -5 and zero from -5.6 on).  Q(t) = exp(-t^2 / 2) R(t), and R as s P(s) with s = 1 / (1 + 0.3 t): P of degree 7 fitted
+// to erfcx(t / sqrt 2) / 2 on 0 .. 16 for the least relative error by reweighted least squares: 2.2e-7, 6e-7 in 32-bit arithmetic.  Past 13 Q is less than 32-bit
+// floats hold.  4096 x 512 x 4096 of bf16 with gelu 38.5 us by erff, 34.2 so (77 by erfcf); its gradient 2048 x 11008 of bf16 39.2, 36.6 so.
+__device__ __forceinline__ float gelu_reach(float z)                    // |z|, 16 at most (NaN stays)
+{
+    float t;
+    asm("min.NaN.f32 %0, %1, 0f41800000;" : "=f"(t) : "f"(fabsf(z)));
+    return t;
+}
+
+__device__ __forceinline__ float gelu_ratio(float t)                    // R(t)
+{
+    const float s = __fdividef(1.0f, fmaf(0.3f, t, 1.0f));
+    float r = 0.0347048553f;
+    r = fmaf(r, s, -0.153187057f);
+    r = fmaf(r, s, 0.199487766f);
+    r = fmaf(r, s, -0.0474263256f);
+    r = fmaf(r, s, 0.125291755f);
+    r = fmaf(r, s, 0.100889287f);
+    r = fmaf(r, s, 0.120600532f);
+    r = fmaf(r, s, 0.119639078f);
+    return r * s;
+}
+
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 template <int ACT>
 __device__ __forceinline__ float activate(float z)
 {
     if (ACT == ESMM_ACT_RELU) return z < 0.0f ? 0.0f : z;   // (NaN stays)
-    if (ACT == ESMM_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118f));
+    if (ACT == ESMM_ACT_GELU) {
+        const float t = gelu_reach(z);
+        return fmaf(-t, __expf(-0.5f * t * t) * gelu_ratio(t), z < 0.0f ? 0.0f : z);
+    }
     if (ACT == ESMM_ACT_GELU_TANH) return __fdividef(z, 1.0f + __expf(-2.0f * GELU_U * z * fmaf(GELU_CUBE * z, z, 1.0f)));
     if (ACT == ESMM_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
     return z;
@@ -103,8 +131,10 @@ template <int ACT>
 __device__ __forceinline__ float activate_grad(float z)
 {
     if (ACT == ESMM_ACT_RELU) return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
-    if (ACT == ESMM_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118f)) + z * __expf(-0.5f * z * z) * 0.3989422804f;
+    if (ACT == ESMM_ACT_GELU) {
+        const float t = gelu_reach(z), e = __expf(-0.5f * t * t), q = e * gelu_ratio(t);
+        return fmaf(copysignf(t, z), e * 0.3989422804f, z < 0.0f ? q : 1.0f - q);
+    }
     if (ACT == ESMM_ACT_GELU_TANH) {
         const float z2 = fminf(z * z, 1e8f);                 // (past it the logistic function is 0 or 1 and its slope 0)
         const float s = logistic(2.0f * GELU_U * z * fmaf(GELU_CUBE, z2, 1.0f));

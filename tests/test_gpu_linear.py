@@ -371,6 +371,45 @@ def test_relu_border_is_not_where_columns_are_small_or_empty(cuda, pkg):
     assert torch.equal(got[0][1].view(torch.int16), got[1][1].view(torch.int16))
 
 
+def tail_error(z):
+    """Relative error of the terms of gelu and its slope in 32 bits: the tail's fit 2.2e-7 (2 steps of 2^-23) and its evaluation 4 of them, the exponential 2 + 1.173 |x|
+    at x = z^2 / 2 and its argument's roundings z^2; a few products: (z^2 1.6 + 11) 2^-23."""
+    return (z * z + 8) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("pair", [0, 256])
+@pytest.mark.parametrize("activation", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_activations_keep_their_negative_tail(cuda, pkg, tuning, t, activation, pair):
+    """Values next to nothing, far left of zero, to the result's last bit: sums of one product are exact."""
+    tuning("LINEAR_PAIR", pair)
+    m, k = 72, 64
+    # (smaller results than 2^-100 are no bf16 matter; gelu_tanh's fall faster)
+    z = torch.linspace(-11.5 if activation == "gelu" else -8.5 if activation == "gelu_tanh" else -60, 6, m * k, device="cuda").view(m, k).to(d.TYPES[t])
+    b, c = torch.eye(k, device="cuda").to(d.TYPES[t]), torch.empty((m, k), dtype=d.TYPES[t], device="cuda")
+    pkg.linear(m, k, k, d.code(pkg, t), z.data_ptr(), b.data_ptr(), d.code(pkg, t), c.data_ptr(), activation=d.act_code(pkg, activation))
+    pkg.device_status()
+    want = d.act(z.double(), activation)
+    # gelu_tanh's argument is a cube: a rounding of it counts about 2 u = 1.6 |z| (1 + 0.045 z^2) times, which is below 7 z^2 here
+    e = tail_error(z.double()) * (1 if activation == "gelu" else 4)
+    u = d.half_step(t)
+    d.assert_close(c, want, (u + e * (1 + u)) * want.abs() + d.smallest(t), "C")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_gelu_gradient_keeps_its_negative_tail(cuda, pkg, t):
+    m, n = 72, 64
+    z = torch.linspace(-11.5, 6, m * n, device="cuda").view(m, n).to(d.TYPES[t])
+    dc, dz = torch.ones_like(z), torch.empty_like(z)
+    pkg.epilogue_backward(m, n, d.code(pkg, t), dc.data_ptr(), z.data_ptr(), pkg.ACT_GELU, dz.data_ptr())
+    pkg.device_status()
+    z = z.double()
+    want = d.act_grad(z, "gelu")
+    terms = 0.5 * torch.special.erfc(-z / 2 ** 0.5) + z.abs() * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    off = tail_error(z) * terms
+    d.assert_close(dz, want, off + d.half_step(t) * (want.abs() + off) + d.smallest(t), "dZ")
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("activation", d.ACTS)
 @pytest.mark.parametrize("m,n", [(1, 8), (9, 264), (1001, 520), (4100, 72)])
