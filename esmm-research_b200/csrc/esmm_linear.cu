@@ -787,11 +787,11 @@ struct LinearSplitEpilogue {
         fetch_rows(p, row0, col, rank * ROWS + threadIdx.x / LANES, split * ROWS, rows);
     }
 
-    // sums: this CTA's, at the same place in every CTA of the cluster
+    // sums: this CTA's, at the same place in every CTA of the cluster.  (The loads from them are volatile, as the cluster barrier is, so that
+    // none is moved before it.)
     template <int SPLIT>
     __device__ __forceinline__ void finish(const LinearParams &p, uint32_t sums, int rank, int row0, int col0, int rows)
     {
-        // (obtained after the cluster barrier, so that no load from them can be moved before it)
         uint32_t part_base[SPLIT];
 #pragma unroll
         for (int part = 0; part < SPLIT; ++part) part_base[part] = SPLIT == 1 ? sums : linear_map_to_cta(sums, (uint32_t)part);
@@ -812,9 +812,9 @@ struct LinearSplitEpilogue {
                     for (int part = 0; part < SPLIT; ++part) {
                         const uint32_t at = part_base[part] + (uint32_t)((ri * (NB + 4) + c) * 4);
                         if constexpr (SPLIT == 1)
-                            asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
                         else
-                            asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u[i][part].x), "=f"(u[i][part].y), "=f"(u[i][part].z), "=f"(u[i][part].w) : "r"(at));
                     }
                 }
 #pragma unroll

@@ -1,6 +1,7 @@
 """CPU tests of the dense operators' entry points: constants of the binding, refusals before any device is touched, workspace sizes, and
 the 64-bit restatements that the GPU tests compare with."""
 import math
+import os
 import re
 
 import pytest
@@ -130,3 +131,16 @@ def test_norm_restatement_against_autograd():
     dx, dw = d.norm_grad(dout, h.detach(), w.detach(), rstd.detach(), dsum)
     assert torch.allclose(x.grad, dx, rtol=1e-12, atol=1e-12) and torch.allclose(w.grad, dw, rtol=1e-12, atol=1e-12)
     assert math.isclose(d.row_scale(torch.zeros(1, 3, dtype=torch.float64))[0].item(), 2.0 ** -100 / 448)
+
+
+def sources(pkg):
+    root = os.path.join(os.path.dirname(pkg.__file__), "csrc")
+    return {f: open(os.path.join(root, f)).read() for f in sorted(os.listdir(root)) if f.endswith((".cu", ".cuh"))}
+
+
+def test_loads_of_what_other_threads_store_stay_behind_their_barriers(pkg):
+    """A shared-memory load in inline assembly reads what others have stored: unless it is volatile, as the barriers are, the compiler may move it across them."""
+    loads = [(name, m) for name, text in sources(pkg).items() for m in re.findall(r'asm[^"]*"ld\.shared[^"]*"', text)]
+    assert len(loads) >= 2
+    for name, m in loads:
+        assert m.startswith("asm volatile"), (name, m)
