@@ -942,7 +942,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
         epilogue.fetch(p, rank, split, row0, col0, rows);
         // The sums of the rows that exist, to shared memory: 16 bytes apart beyond their length, so that the stores of eight threads
         // (eight rows) fall on all banks.  The ring is free: every copy has landed and every MMA has read it.
-        ok = mbar_wait(accf, 0, abort_flag);
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(accf, 0, abort_flag));   // (the loads from tensor memory are the whole warp's)
         const int q = warp & 3, c0 = (warp >> 2) * (NB / 2);      // TMEM lanes 32 q .., columns c0 ..
         if (ok && q * 32 < rows) {
             linear_fence_after();

@@ -144,3 +144,13 @@ def test_loads_of_what_other_threads_store_stay_behind_their_barriers(pkg):
     assert len(loads) >= 2
     for name, m in loads:
         assert m.startswith("asm volatile"), (name, m)
+
+
+def test_a_warp_agrees_on_its_wait_before_its_tensor_core_instructions(pkg):
+    """A bounded wait may pass in one lane and run out in another; what is the whole warp's (sync.aligned) comes only after a vote."""
+    text = sources(pkg)["esmm_linear.cu"]
+    waits = [m.start() for m in re.finditer(r"[^_]mbar_wait\(", text)]
+    assert len(waits) >= 6
+    for at in waits:
+        after = re.search(r"linear_tmem_ld\(|linear_mma_step<|linear_load_step<|linear_commit<", text[at:])
+        assert after is None or "__all_sync" in text[text.rfind("\n", 0, at):at + after.start()], text[at:at + 60]
