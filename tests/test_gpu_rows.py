@@ -187,6 +187,22 @@ def test_norm_backward(cuda, pkg, t, m, k):
     assert torch.equal(dx2, dsum)
 
 
+# Many more rows than are under way in a CTA at once: one warp per row, a CTA per row that keeps it in registers, one that reads its slot again (16-bit K past 8192, FP32
+# past 4096), and rows that are no whole vectors with four, eight and sixteen elements per thread.
+MANY_ROWS = [(40000, 64), (20000, 512), (5000, 4096), (1500, 8192), (1500, 16384), (5000, 1501), (2500, 4001), (1300, 6091)]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,k", MANY_ROWS)
+def test_norm_backward_of_many_rows(cuda, pkg, t, m, k):
+    test_norm_backward(cuda, pkg, t, m, k)
+
+
+@pytest.mark.parametrize("m,k", MANY_ROWS)
+def test_norm_backward_of_many_rows_over_its_inputs(cuda, pkg, m, k):
+    test_norm_backward_over_its_inputs(cuda, pkg, m, k)
+
+
 def test_norm_gradient_against_differences(cuda, pkg):
     m, k = 6, 96
     x, _, w, dout, _ = tensors(m, k, "f32", seed=7)
