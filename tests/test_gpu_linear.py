@@ -111,6 +111,18 @@ def test_parts_of_k(cuda, pkg, tuning, split, columns):
         check(pkg, m, n, k, t, out="bf16" if t == "e4m3" else t, bias=True, residual=True, scales=True)
 
 
+@pytest.mark.parametrize("split", [4, 5, 6, 7])
+@pytest.mark.parametrize("columns", [64, 128])
+def test_other_parts_of_k(cuda, pkg, tuning, split, columns):
+    """The numbers of parts that the library chooses beside those above, and the odd ones that only the hook asks for; K steps that do not divide among them."""
+    tuning("LINEAR_PAIR", 0)
+    tuning("LINEAR_SPLIT", split)
+    tuning("LINEAR_COLUMNS", columns)
+    for t, (m, n, k) in [("bf16", (5, 136, 1000)), ("bf16", (200, 264, 72)), ("e4m3", (130, 72, 2064)), ("f16", (128, 320, 640)), ("bf16", (17, 128, 4160))]:
+        check(pkg, m, n, k, t, out="bf16" if t == "e4m3" else t, bias=True, residual=True, scales=True, pre=True, activation="silu")
+        check(pkg, m, n, k, t, out="bf16" if t == "e4m3" else t)
+
+
 @pytest.mark.parametrize("activation", d.ACTS)
 @pytest.mark.parametrize("pair", [0, 256])
 def test_epilogue_parts(cuda, pkg, tuning, activation, pair):
@@ -408,6 +420,26 @@ def test_gelu_gradient_keeps_its_negative_tail(cuda, pkg, t):
     terms = 0.5 * torch.special.erfc(-z / 2 ** 0.5) + z.abs() * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
     off = tail_error(z) * terms
     d.assert_close(dz, want, off + d.half_step(t) * (want.abs() + off) + d.smallest(t), "dZ")
+
+
+@pytest.mark.parametrize("m,n,k", [(24, 40, 32), (40, 24, 64)])
+def test_gradients_against_differences_along_themselves(cuda, pkg, m, n, k):
+    """The slope of <dc, C> along the signs of its gradient, by differences in 64 bits: a sum of the gradient's magnitudes, of which the roundings are a small share."""
+    s = layer_state(pkg, m, n, k, seed=5)
+    layer_calls(pkg, s, 0)
+    pkg.device_status()
+    a, b, dc, bias = s["a"].double(), s["b"].double(), s["dc"].double(), s["bias"].double()
+    f = lambda x, w: (dc * d.act(x @ w + bias, "gelu_tanh")).sum()  # noqa: E731
+    z = a @ b + bias
+    slopes = dc * d.act_grad(z, "gelu_tanh")
+    for key, grad in (("da", slopes @ b.t()), ("db", a.t() @ slopes)):
+        v, h = torch.sign(grad), 1e-6
+        slope = (f(a + h * v, b) - f(a - h * v, b) if key == "da" else f(a, b + h * v) - f(a, b - h * v)) / (2 * h)
+        # half a step of bf16, 2^-8, each of pre (times a second derivative of at most 1.2), of dZ and of the gradient itself, against the sums of magnitudes
+        share = 2.0 ** -8 * (slopes.abs() + dc.abs() * 1.2 * z.abs())
+        tol = (share @ b.abs().t() if key == "da" else a.abs().t() @ share).sum() + 2.0 ** -8 * grad.abs().sum()
+        assert tol <= 0.15 * slope.abs(), (key, tol, slope)
+        assert abs((s[key].double() * v).sum() - slope) <= tol, (key, slope)
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
