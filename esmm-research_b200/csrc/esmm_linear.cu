@@ -345,7 +345,7 @@ __device__ __noinline__ int linear_note_border(const LinearParams &p, const char
             noted = 0;
         }
         for (; rows && left > 0; rows &= rows - 1, --left, ++noted)
-            if (lane == 0) list[noted] = make_int2(row0 + __ffs((int)rows) - 1, col0 + j);
+            if (lane == 0 && bounds_ok(noted < LP_LIST, p.status, 66)) list[noted] = make_int2(row0 + __ffs((int)rows) - 1, col0 + j);
     }
     return noted;
 }
@@ -953,7 +953,7 @@ esmm_linear_split_kernel(const __grid_constant__ LinearMaps maps, const __grid_c
                 float z[32];
                 linear_tmem_ld(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(c0 + c), z);
                 linear_tmem_wait(z);
-                if (mine) {
+                if (mine && bounds_ok(ls_red_bytes(q * 32 + lane, NB) + (c0 + c + 32) * 4 <= bar_off, p.status, 77)) {   // checked build: site 77
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(red + c + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
                 }

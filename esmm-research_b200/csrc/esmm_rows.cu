@@ -161,7 +161,7 @@ esmm_rmsnorm_kernel(const NormParams p)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (threadIdx.x + i * blockDim.x) * VEC;
-            if (c < p.K) {
+            if (c < p.K && bounds_ok(base + c + VEC <= end, p.status, 59)) {   // checked build: site 59
                 xr[i] = load_raw<T, VEC>(x + c);
                 if (res) rr[i] = load_raw<T, VEC>(res + c);
             }
@@ -258,13 +258,22 @@ esmm_rmsnorm_ragged_kernel(const NormParams p)
     auto whole = [&](int i) { return off(i) >= lead && off(i) + VEC <= p.K + lead; };
     auto in = [&](int i, int j) { return off(i) + j >= lead && off(i) + j < p.K + lead; };
     auto loadable = [&](int i) { return (size_t)(off(i) + VEC) <= left; };   // the matrix does not end inside it
+    // checked build, sites 67 (vectors), 68 (elements), 69 (weights), 70 (results): `n` elements from element j of vector i lie in the row, or, with their neighbours, in the matrix
+    auto in_row = [&](int i, int j, int n, int site) {
+        if constexpr (kCheckedBuild) return bounds_ok(first + off(i) + j >= begin && first + off(i) + j + n <= begin + p.K && row < (size_t)p.M, p.status, site);
+        return true;
+    };
+    auto in_matrix = [&](int i) {
+        if constexpr (kCheckedBuild) return bounds_ok(first + off(i) + VEC <= (size_t)p.M * p.K, p.status, 67);
+        return true;
+    };
     float h[NV][VEC];
     float ss = 0.0f;
     {
         raw_t xr[NV], rr[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (here(i) && loadable(i)) {
+            if (here(i) && loadable(i) && in_matrix(i)) {
                 xr[i] = load_raw<T, VEC>(x + off(i));
                 if (res) rr[i] = load_raw<T, VEC>(res + off(i));
             }
@@ -284,15 +293,15 @@ esmm_rmsnorm_ragged_kernel(const NormParams p)
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (in(i, j)) h[i][j] = to_float<T>(x[off(i) + j]) + (res ? to_float<T>(res[off(i) + j]) : 0.0f);
+                    if (in(i, j) && in_row(i, j, 1, 68)) h[i][j] = to_float<T>(x[off(i) + j]) + (res ? to_float<T>(res[off(i) + j]) : 0.0f);
             }
             T *to = static_cast<T *>(p.sum) + first + off(i);
             if (whole(i)) {
-                if (NORM && p.sum) store_raw<T, VEC>(to, h[i]);
+                if (NORM && p.sum && in_row(i, 0, VEC, 70)) store_raw<T, VEC>(to, h[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    if (NORM && p.sum && in(i, j)) to[j] = from_float<T>(h[i][j]);
+                    if (NORM && p.sum && in(i, j) && in_row(i, j, 1, 70)) to[j] = from_float<T>(h[i][j]);
                     if (!in(i, j)) h[i][j] = 0.0f;                   // (counts for nothing from here on)
                 }
             }
@@ -309,6 +318,7 @@ esmm_rmsnorm_ragged_kernel(const NormParams p)
             if (!weight || !here(i)) continue;
             const T *from = weight + (off(i) - lead);
             if (whole(i)) {
+                if (!in_row(i, 0, VEC, 69)) continue;
                 if (VEC == 8 && (lead & 1) == 0) {                   // pairs on their own alignment
                     const uint32_t *pairs = reinterpret_cast<const uint32_t *>(from);
 #pragma unroll
@@ -323,7 +333,7 @@ esmm_rmsnorm_ragged_kernel(const NormParams p)
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (in(i, j)) w[i][j] = to_float<T>(from[j]);
+                    if (in(i, j) && in_row(i, j, 1, 69)) w[i][j] = to_float<T>(from[j]);
             }
         }
         ss = row_reduce<false>(ss, slots);
@@ -356,20 +366,20 @@ esmm_rmsnorm_ragged_kernel(const NormParams p)
             for (int j = 0; j < VEC; ++j) h[i][j] = e4m3_quotient(h[i][j], scale, inv);
             uint8_t *to = static_cast<uint8_t *>(p.out) + first + off(i);
             if (whole(i)) {
-                store_e4m3<VEC>(to, h[i]);
+                if (in_row(i, 0, VEC, 70)) store_e4m3<VEC>(to, h[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (in(i, j)) to[j] = (uint8_t)pack_e4m3(h[i][j], 0.0f);
+                    if (in(i, j) && in_row(i, j, 1, 70)) to[j] = (uint8_t)pack_e4m3(h[i][j], 0.0f);
             }
         } else {
             T *to = static_cast<T *>(p.out) + first + off(i);
             if (whole(i)) {
-                store_raw<T, VEC>(to, h[i]);
+                if (in_row(i, 0, VEC, 70)) store_raw<T, VEC>(to, h[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (in(i, j)) to[j] = from_float<T>(h[i][j]);
+                    if (in(i, j) && in_row(i, j, 1, 70)) to[j] = from_float<T>(h[i][j]);
             }
         }
     }
@@ -388,7 +398,8 @@ esmm_rmsnorm_long_kernel(const NormParams p)
     const T *x = static_cast<const T *>(p.x) + base;
     const T *res = p.residual ? static_cast<const T *>(p.residual) + base : nullptr;
     const T *weight = static_cast<const T *>(p.weight);
-    auto h_at = [&](int c) { return to_float<T>(x[c]) + (res ? to_float<T>(res[c]) : 0.0f); };
+    auto inside = [&](int c) { return bounds_ok(base + c < (size_t)p.M * p.K && c < p.K, p.status, 71); };   // checked build: site 71
+    auto h_at = [&](int c) { return inside(c) ? to_float<T>(x[c]) + (res ? to_float<T>(res[c]) : 0.0f) : 0.0f; };
     float rstd = 1.0f;
     if (NORM) {
         float ss = 0.0f;
@@ -409,6 +420,7 @@ esmm_rmsnorm_long_kernel(const NormParams p)
     }
     for (int c = threadIdx.x; c < p.K; c += blockDim.x) {
         const float h = h_at(c), y = y_at(h, c);
+        if (!inside(c)) continue;
         if (NORM && p.sum) static_cast<T *>(p.sum)[base + c] = from_float<T>(h);
         if (OUT8) static_cast<uint8_t *>(p.out)[base + c] = (uint8_t)pack_e4m3(e4m3_quotient(y, scale, inv), 0.0f);
         else static_cast<T *>(p.out)[base + c] = from_float<T>(y);
@@ -557,7 +569,7 @@ esmm_rmsnorm_backward_kernel(const NormGradParams p)
         settle_after_timeout();
         if ((threadIdx.x & 31) == 0) atomicExch(p.status, (int)ESMM_ERR_TIMEOUT);
     }
-    if (!p.partial) return;
+    if (!p.partial || !bounds_ok((int)blockIdx.x < min(p.M, ROWS_MAX_PARTIALS), p.status, 72)) return;   // checked build: site 72
     float *to = p.partial + (size_t)blockIdx.x * p.K;
     float *mine = groups == 1 ? to : reinterpret_cast<float *>(smem) + (size_t)group * (blockDim.x * NV * VEC);
     if (groups > 1) __syncthreads();               // (every group's rows are through: the rings' memory is free)
@@ -605,7 +617,7 @@ esmm_rmsnorm_backward_ragged_kernel(const NormGradParams p)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = threadIdx.x + i * blockDim.x;
-            if (c < p.K) {
+            if (c < p.K && bounds_ok(base + c < (size_t)p.M * p.K, p.status, 73)) {   // checked build: site 73
                 g_raw[i] = dout[base + c];
                 h_raw[i] = h[base + c];
                 if (dsum) s_raw[i] = dsum[base + c];
@@ -645,7 +657,7 @@ esmm_rmsnorm_backward_ragged_kernel(const NormGradParams p)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = threadIdx.x + i * blockDim.x;
-            if (c < p.K) p.partial[(size_t)blockIdx.x * p.K + c] = dw[i];
+            if (c < p.K && bounds_ok((int)blockIdx.x < min(p.M, ROWS_MAX_PARTIALS), p.status, 72)) p.partial[(size_t)blockIdx.x * p.K + c] = dw[i];
         }
     }
 }
@@ -659,7 +671,8 @@ esmm_rmsnorm_backward_long_kernel(const NormGradParams p)
     grid_dependency_wait();
     __shared__ float slots[64];
     const T *weight = static_cast<const T *>(p.weight);
-    float *to = p.partial ? p.partial + (size_t)blockIdx.x * p.K : nullptr;
+    float *to = p.partial && bounds_ok((int)blockIdx.x < min(p.M, ROWS_MAX_PARTIALS), p.status, 72) ? p.partial + (size_t)blockIdx.x * p.K : nullptr;
+    auto inside = [&](size_t base, int c) { return bounds_ok(base + c < (size_t)p.M * p.K && c < p.K, p.status, 71); };
     int turn = 0;
     for (size_t row = blockIdx.x; row < (size_t)p.M; row += gridDim.x, turn ^= 32) {
         const size_t base = row * (size_t)p.K;
@@ -667,10 +680,10 @@ esmm_rmsnorm_backward_long_kernel(const NormGradParams p)
         const T *dsum = p.dsum ? static_cast<const T *>(p.dsum) + base : nullptr;
         const float rstd = p.rstd[row];
         float dot = 0.0f;
-        for (int c = threadIdx.x; c < p.K; c += blockDim.x)
+        for (int c = threadIdx.x; c < p.K && inside(base, c); c += blockDim.x)
             dot = fmaf(to_float<T>(dout[c]) * (weight ? to_float<T>(weight[c]) : 1.0f), to_float<T>(h[c]) * rstd, dot);
         dot = row_reduce<false>(dot, slots + turn) / (float)p.K;
-        for (int c = threadIdx.x; c < p.K; c += blockDim.x) {
+        for (int c = threadIdx.x; c < p.K && inside(base, c); c += blockDim.x) {
             const float g = to_float<T>(dout[c]), xh = to_float<T>(h[c]) * rstd;
             if (to) to[c] = row == blockIdx.x ? g * xh : fmaf(g, xh, to[c]);
             const float gw = g * (weight ? to_float<T>(weight[c]) : 1.0f);
@@ -683,7 +696,7 @@ esmm_rmsnorm_backward_long_kernel(const NormGradParams p)
 // ..., the 64 sums are added as a tree.
 template <typename T>
 __global__ void __launch_bounds__(512)
-esmm_column_sum_kernel(const float *partial, int rows, int K, T *out)
+esmm_column_sum_kernel(const float *partial, int rows, int K, T *out, int *status)
 {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -696,6 +709,7 @@ esmm_column_sum_kernel(const float *partial, int rows, int K, T *out)
     auto take = [&](float4 &sum, int r) {
         const float *at = partial + (size_t)r * K + c;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!bounds_ok(r < min(rows, ROWS_MAX_PARTIALS), status, 74)) return;   // checked build: site 74
         if (vectors) {
             if (c < K) v = *reinterpret_cast<const float4 *>(at);
         } else {
@@ -725,7 +739,7 @@ esmm_column_sum_kernel(const float *partial, int rows, int K, T *out)
     for (int i = 0; i < 2; ++i) {                 // a warp adds up two of the 32 columns
         const int col = warp * 2 + i;
         const float v = warp_sum(sums[lane][col] + sums[lane + 32][col]);
-        if (lane == 0 && blockIdx.x * 32 + col < K) out[blockIdx.x * 32 + col] = from_float<T>(v);
+        if (lane == 0 && blockIdx.x * 32 + col < K && bounds_ok((size_t)blockIdx.x * 32 + col < (size_t)K, status, 74)) out[blockIdx.x * 32 + col] = from_float<T>(v);
     }
 }
 
@@ -760,7 +774,7 @@ esmm_epilogue_backward_kernel(const EpiGradParams p)
             raw_t g[U], z[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + 8 * u < r1) {
+                if (r + 8 * u < r1 && bounds_ok((size_t)(r + 8 * u) * p.N + col + VEC <= (size_t)p.M * p.N, p.status, 63)) {
                     g[u] = load_raw<T, VEC>(dc + (size_t)(r + 8 * u) * p.N + col);
                     if (pre) z[u] = load_raw<T, VEC>(pre + (size_t)(r + 8 * u) * p.N + col);
                 }
@@ -793,7 +807,7 @@ esmm_epilogue_backward_kernel(const EpiGradParams p)
             float s = 0.0f;
 #pragma unroll
             for (int w = 0; w < 8; ++w) s += sums[w][c];
-            if (to < p.N) p.partial[(size_t)blockIdx.y * p.N + to] = s;
+            if (to < p.N && bounds_ok((int)blockIdx.y < min((p.M + 7) / 8, ROWS_MAX_PARTIALS), p.status, 72)) p.partial[(size_t)blockIdx.y * p.N + to] = s;
         }
     }
 }
@@ -802,7 +816,7 @@ esmm_epilogue_backward_kernel(const EpiGradParams p)
 // scale[n] = amax_k |B[k][n]| / 448: 32 columns per CTA, 32 rows at a time.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-esmm_column_scale_kernel(const T *B, int K, int N, float *scale)
+esmm_column_scale_kernel(const T *B, int K, int N, float *scale, int *status)
 {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -810,18 +824,18 @@ esmm_column_scale_kernel(const T *B, int K, int N, float *scale)
     const int n = blockIdx.x * 32 + threadIdx.x;
     float amax = 0.0f;
     if (n < N)
-        for (int k = threadIdx.y; k < K; k += 32) amax = fmaxf(amax, fabsf(to_float<T>(B[(size_t)k * N + n])));
+        for (int k = threadIdx.y; k < K && bounds_ok((size_t)k * N + n < (size_t)K * N, status, 75); k += 32) amax = fmaxf(amax, fabsf(to_float<T>(B[(size_t)k * N + n])));
     part[threadIdx.y][threadIdx.x] = amax;
     __syncthreads();
     amax = warp_max(part[threadIdx.x][threadIdx.y]);
     const int to = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && to < N) scale[to] = e4m3_scale(amax);
+    if (threadIdx.x == 0 && to < N && bounds_ok(to >= 0, status, 75)) scale[to] = e4m3_scale(amax);   // checked build: site 75
 }
 
 // bt[n][k] = e4m3(B[k][n] / scale[n]): tiles of 128 k x 32 n through shared memory, four codes of a row per store
 template <typename T>
 __global__ void __launch_bounds__(256)
-esmm_quantize_transpose_kernel(const T *B, int K, int N, const float *scale, uint8_t *bt)
+esmm_quantize_transpose_kernel(const T *B, int K, int N, const float *scale, uint8_t *bt, int *status)
 {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -830,11 +844,11 @@ esmm_quantize_transpose_kernel(const T *B, int K, int N, const float *scale, uin
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float sc = n0 + lane < N ? scale[n0 + lane] : 1.0f, inv = 1.0f / sc;
     for (int r = warp; r < 128; r += 8)
-        tile[r][lane] = k0 + r < K && n0 + lane < N ? e4m3_quotient(to_float<T>(B[(size_t)(k0 + r) * N + n0 + lane]), sc, inv) : 0.0f;
+        tile[r][lane] = k0 + r < K && n0 + lane < N && bounds_ok((size_t)(k0 + r) * N + n0 + lane < (size_t)K * N, status, 76) ? e4m3_quotient(to_float<T>(B[(size_t)(k0 + r) * N + n0 + lane]), sc, inv) : 0.0f;
     __syncthreads();
     for (int c = warp; c < 32; c += 8) {
         const int n = n0 + c, k = k0 + lane * 4;
-        if (n < N && k < K)   // (K is a multiple of 16)
+        if (n < N && k < K && bounds_ok((size_t)n * K + k + 4 <= (size_t)N * K, status, 76))   // (K is a multiple of 16; checked build: site 76)
             *reinterpret_cast<uint32_t *>(bt + (size_t)n * K + k) =
                 pack_e4m3(tile[lane * 4][c], tile[lane * 4 + 1][c]) | (pack_e4m3(tile[lane * 4 + 2][c], tile[lane * 4 + 3][c]) << 16);
     }
@@ -996,12 +1010,12 @@ static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas
     return ESMM_OK;
 }
 
-static int column_sum(const float *partial, int rows, int K, int dtype, void *out, cudaStream_t stream)
+static int column_sum(const float *partial, int rows, int K, int dtype, void *out, int *status, cudaStream_t stream)
 {
     auto go = [&](auto tag) -> int {
         typedef decltype(tag) T;
         ESMM_CUDA_TRY(launch_dependent(esmm_column_sum_kernel<T>, dim3((unsigned)ceil_div(K, 32)), dim3(8, 64), 0, stream, partial, rows, K,
-                                       static_cast<T *>(out)));
+                                       static_cast<T *>(out), status));
         return ESMM_OK;
     };
     return dtype == ESMM_F32 ? go(float()) : dtype == ESMM_F16 ? go(__half()) : go(__nv_bfloat16());
@@ -1102,7 +1116,7 @@ int esmm_rmsnorm_backward(int M, int K, int dtype, const void *d_dout, const voi
     else if (dtype == ESMM_F16) st = norm_backward_type<__half>(p, aligned, sms, &ctas, stream);
     else st = norm_backward_type<__nv_bfloat16>(p, aligned, sms, &ctas, stream);
     if (st != ESMM_OK || !d_dweight) return st;
-    return column_sum(p.partial, ctas, K, dtype, d_dweight, stream);
+    return column_sum(p.partial, ctas, K, dtype, d_dweight, p.status, stream);
 }
 
 size_t esmm_epilogue_backward_workspace_bytes(int M, int N)
@@ -1150,7 +1164,7 @@ int esmm_epilogue_backward(int M, int N, int dtype, const void *d_dC, const void
                     : dtype == ESMM_F16 ? go(esmm_epilogue_backward_kernel<__half>)
                                         : go(esmm_epilogue_backward_kernel<__nv_bfloat16>);
     if (lst != ESMM_OK || !d_dbias) return lst;
-    return column_sum(p.partial, runs, N, dtype, d_dbias, stream);
+    return column_sum(p.partial, runs, N, dtype, d_dbias, p.status, stream);
 }
 
 int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float *d_scale, void *stream_)
@@ -1162,12 +1176,14 @@ int esmm_quantize_b(int K, int N, int dtype, const void *d_B, void *d_bt, float 
     if (!row_dtype(dtype)) return ESMM_ERR_UNSUPPORTED;
     if (!element_aligned(d_B, dtype_bytes(dtype)) || ((uintptr_t)d_bt & 15) || !element_aligned(d_scale, 4)) return ESMM_ERR_ALIGN;
     if (K / 128 >= 65535 || N > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
+    int *status = device_status_ptr();
+    if (!status) return ESMM_ERR_CUDA;
     auto go = [&](auto tag) -> int {
         typedef decltype(tag) T;
         const T *B = static_cast<const T *>(d_B);
-        ESMM_CUDA_TRY(launch_dependent(esmm_column_scale_kernel<T>, dim3((unsigned)ceil_div(N, 32)), dim3(32, 32), 0, stream, B, K, N, d_scale));
+        ESMM_CUDA_TRY(launch_dependent(esmm_column_scale_kernel<T>, dim3((unsigned)ceil_div(N, 32)), dim3(32, 32), 0, stream, B, K, N, d_scale, status));
         ESMM_CUDA_TRY(launch_dependent(esmm_quantize_transpose_kernel<T>, dim3((unsigned)ceil_div(N, 32), (unsigned)ceil_div(K, 128)), dim3(256),
-                                       0, stream, B, K, N, (const float *)d_scale, static_cast<uint8_t *>(d_bt)));
+                                       0, stream, B, K, N, (const float *)d_scale, static_cast<uint8_t *>(d_bt), status));
         return ESMM_OK;
     };
     return dtype == ESMM_F32 ? go(float()) : dtype == ESMM_F16 ? go(__half()) : go(__nv_bfloat16());

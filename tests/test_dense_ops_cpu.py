@@ -154,3 +154,13 @@ def test_a_warp_agrees_on_its_wait_before_its_tensor_core_instructions(pkg):
     for at in waits:
         after = re.search(r"linear_tmem_ld\(|linear_mma_step<|linear_load_step<|linear_commit<", text[at:])
         assert after is None or "__all_sync" in text[text.rfind("\n", 0, at):at + after.start()], text[at:at + 60]
+
+
+def test_every_row_kernel_is_checked_in_the_checked_build(pkg):
+    """Kernels whose indices depend on the sizes have bounds checks for -DESMM_CHECKED, each kind of access under a number of its own."""
+    text = sources(pkg)["esmm_rows.cu"]
+    kernels = text.split("__global__")[1:]
+    assert len(kernels) == 10
+    for body in kernels:
+        body = body[:body.index("\n}\n")]
+        assert "bounds_ok(" in body, body.split("\n")[1]
