@@ -1037,7 +1037,7 @@ int esmm_rmsnorm(int M, int K, int dtype, const void *d_x, const void *d_residua
     const int size = dtype_bytes(dtype);
     for (const void *q : {d_x, d_residual, d_weight, (const void *)d_sum, (const void *)(out8 ? nullptr : d_out)})
         if (!element_aligned(q, size)) return ESMM_ERR_ALIGN;
-    if (!element_aligned(d_scale, 4) || !element_aligned(d_rstd, 4)) return ESMM_ERR_ALIGN;
+    if ((out8 && !element_aligned(d_scale, 4)) || !element_aligned(d_rstd, 4)) return ESMM_ERR_ALIGN;
     NormParams p;
     memset(&p, 0, sizeof p);
     p.M = M;
@@ -1094,7 +1094,7 @@ int esmm_rmsnorm_backward(int M, int K, int dtype, const void *d_dout, const voi
     const int size = dtype_bytes(dtype);
     for (const void *q : {d_dout, d_h, d_weight, d_dsum, (const void *)d_dx, (const void *)d_dweight})
         if (!element_aligned(q, size)) return ESMM_ERR_ALIGN;
-    if (!element_aligned(d_rstd, 4) || ((uintptr_t)d_workspace & 15)) return ESMM_ERR_ALIGN;
+    if (!element_aligned(d_rstd, 4) || (d_dweight && ((uintptr_t)d_workspace & 15))) return ESMM_ERR_ALIGN;
     NormGradParams p;
     memset(&p, 0, sizeof p);
     p.M = M;
@@ -1136,7 +1136,8 @@ int esmm_epilogue_backward(int M, int N, int dtype, const void *d_dC, const void
     const int vec = 16 / dtype_bytes(dtype);
     if (M <= 0 || N <= 0 || N % vec) return ESMM_ERR_SHAPE;
     if (M > MAX_EXTENT || N > MAX_EXTENT) return ESMM_ERR_TOO_LARGE;
-    if (!aligned16({d_dC, d_pre, d_dZ, d_workspace}) || !element_aligned(d_dbias, dtype_bytes(dtype))) return ESMM_ERR_ALIGN;
+    if (!aligned16({d_dC, activation == ESMM_ACT_NONE ? nullptr : d_pre, d_dZ, d_dbias ? d_workspace : nullptr}) || !element_aligned(d_dbias, dtype_bytes(dtype)))
+        return ESMM_ERR_ALIGN;
     EpiGradParams p;
     memset(&p, 0, sizeof p);
     p.M = M;

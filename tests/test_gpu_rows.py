@@ -271,6 +271,24 @@ def test_feed_forward_block_in_8_bits(cuda, pkg, m):
     d.assert_close(out, want, off + ub * (want.abs() + off))
 
 
+def test_pointers_that_a_call_does_not_use_may_lie_anywhere(cuda, pkg):
+    """d_scale without e4m3, d_workspace without the weight's or bias's gradient, d_pre without an activation."""
+    m, k = 12, 64
+    x, _, w, dout, _ = tensors(m, k, "bf16", seed=9)
+    odd = torch.zeros(4096, dtype=torch.uint8, device="cuda")[1:].data_ptr()
+    rstd = torch.empty(m, device="cuda")
+    got = []
+    for unused in (0, odd):
+        out, dx, dz = (torch.empty_like(x) for _ in range(3))
+        pkg.rmsnorm(m, k, pkg.BF16, x.data_ptr(), 0, w.data_ptr(), EPS, 0, pkg.BF16, out.data_ptr(), unused, rstd.data_ptr())
+        pkg.rmsnorm_backward(m, k, pkg.BF16, dout.data_ptr(), x.data_ptr(), w.data_ptr(), rstd.data_ptr(), 0, dx.data_ptr(), 0, unused)
+        pkg.epilogue_backward(m, k, pkg.BF16, dout.data_ptr(), unused, pkg.ACT_NONE, dz.data_ptr(), 0, unused)
+        pkg.device_status()
+        got.append((out, dx, dz))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_norm_captured_and_replayed_with_new_inputs(cuda, pkg):
     m, k = 300, 1032
     sets = [tensors(m, k, "bf16", seed=s) for s in (11, 12)]
