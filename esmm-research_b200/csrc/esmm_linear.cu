@@ -250,6 +250,7 @@ static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
 // warps with a part of K each.  us with the values kept, silu / relu: 520 x 776 x 1032 fp16 9.2 / 11.1 (13.8 where an element is found), 2048 x 4096 x 11008 131 / 211
 // (some 800 elements, a column of B being 4096 lines of memory); summed by the warp alone within the piece 418, by a kernel of its own 220, and 17.5 for the small one.
 constexpr float LB_SHARE = 6e-9f, LB_SHARE_F8 = 3e-10f;
+constexpr float LB_WIDEST = 1e-3f;            // (from K = 167 thousand on, where 64-bit sums of all that may be off would take longer than the product)
 constexpr int LB_MOST = LP_LIST / 2;          // elements per piece: more are no coincidence, and a bound on the time
 constexpr int LB_ROWS = 8;                    // in fewer rows a column's size does not show: the row's is taken alone
 
@@ -1176,7 +1177,7 @@ extern "C" int esmm_linear(int M, int N, int K, int dtype, const void *d_A, int 
 
     const bool border = d_pre && activation == ESMM_ACT_RELU;
     if (border) {
-        p.border = (float)K * (f8 ? LB_SHARE_F8 : LB_SHARE);
+        p.border = std::min((float)K * (f8 ? LB_SHARE_F8 : LB_SHARE), LB_WIDEST);
         p.K = K;
         p.A = d_A;
         p.B = d_B;

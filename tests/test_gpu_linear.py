@@ -327,6 +327,13 @@ def test_relu_keeps_the_sign_of_sums_next_to_zero(cuda, pkg, t, trans, half, m, 
     assert torch.equal(dz[at], torch.where(z[at] > 0, dc[at], torch.zeros_like(dc[at])))
 
 
+@pytest.mark.parametrize("t,trans,half", [("f16", "nn", 512), ("bf16", "nt", 2048), ("e4m3", "nt", 520)])
+@pytest.mark.parametrize("m,n", [(6, 136), (294, 104), (38, 1064)])
+def test_relu_border_in_few_rows(cuda, pkg, t, trans, half, m, n):
+    """A piece of six rows, by itself and below others, where a column's size does not show; columns that end inside a piece."""
+    test_relu_keeps_the_sign_of_sums_next_to_zero(cuda, pkg, t, trans, half, m // 8 * 8 if trans == "tn" else m, n, False)
+
+
 def test_relu_border_beside_biases(cuda, pkg):
     """Sums that a bias of size one swallows are not the zeros of pruned blocks: elements next to zero in their rows and columns keep their side."""
     m, n = 296, 1032
