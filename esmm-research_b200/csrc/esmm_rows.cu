@@ -994,8 +994,8 @@ static int norm_backward_type(NormGradParams p, bool aligned, int sms, int *ctas
         constexpr int N = decltype(nv)::value;
         auto *kernel = esmm_rmsnorm_backward_ragged_kernel<T, N>;
         const int threads = ceil_div(ceil_div(p.K, N), 32) * 32;
-        // (1024 threads of an SM: what a kernel of up to 64 registers has room for; sixteen elements need more, and their 512 threads
-        // are alone)
+        // (1024 threads of an SM: what a kernel of up to 64 registers has room for; sixteen elements need more, 60 bytes a thread beyond the 128
+        // there are, and their 512 threads are alone)
         *ctas = std::max(1, std::min(std::min(p.M, ROWS_MAX_PARTIALS), sms * std::max(1, std::min((N > 8 ? 512 : 1024) / threads, 4))));
         ESMM_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)*ctas), dim3(threads), 0, stream, p));
         return ESMM_OK;

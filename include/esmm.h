@@ -231,7 +231,7 @@ int esmm_selftest_bounded_wait(unsigned budget_us, void *stream);
  * Names: TILE_M (64 | 128), STAGES, BROW_BITS, ROW_DENSITY, FORCE_LISTED, NO_RUN_TILES, VEC_PATTERNS
  * (0 | 4 | 16), NO_SKINNY, SKINNY_ROWS (16 | 32), PRODUCER_WARPS (3 | 7 | 0: pins the tiled kernel's launch shape),
  * BLOCK_MODE (0 | 1: pins the tiled kernel's way of working, see esmm_gemm_blocks.cuh; -1: its own rule, also in short launches), NO_DEPENDENT_LAUNCH, GROUP_M, GRID, TF32_PAIR (0 | 128 | 256), TF32_SPLIT_LAST,
- * TF32_DIRECT_STORES, LINEAR_PAIR (0 | 64 | 128 | 192 | 256, 288 .. 512 where one round of such tiles takes all of C), LINEAR_TAIL (64 | 128 | 192), LINEAR_SPLIT (1 .. 8) and LINEAR_COLUMNS (64 | 128), which pin esmm_linear's kernel and tile widths, the parts of K and the other kernel's tile width, and SWIZZLE and PACK, which are accepted and without effect (the kernels they were for are gone).  esmm_tuning_set returns ESMM_ERR_UNSUPPORTED for any other name;
+ * TF32_DIRECT_STORES, LINEAR_PAIR (0 | 64 | 128 | 192 | 256; 288 .. 512 in steps of 32, of 64 where B is stored K x N, where one round of such tiles takes all of C; relu with d_pre: 64 .. 256 only; without effect otherwise), LINEAR_TAIL (64 | 128 | 192), LINEAR_SPLIT (1 .. 8) and LINEAR_COLUMNS (64 | 128), which pin esmm_linear's kernel and tile widths, the parts of K and the other kernel's tile width, and SWIZZLE and PACK, which are accepted and without effect (the kernels they were for are gone).  esmm_tuning_set returns ESMM_ERR_UNSUPPORTED for any other name;
  * esmm_tuning_reset returns every hook to "unset" (the library's own choice).
  */
 int esmm_tuning_set(const char *name, int value);
