@@ -334,6 +334,36 @@ def test_relu_border_in_few_rows(cuda, pkg, t, trans, half, m, n):
     test_relu_keeps_the_sign_of_sums_next_to_zero(cuda, pkg, t, trans, half, m // 8 * 8 if trans == "tn" else m, n, False)
 
 
+def test_relu_border_captured_and_on_two_streams(cuda, pkg):
+    """A captured product with new operands at every replay, beside one on another stream."""
+    m, n, k = 296, 264, 1040
+    sets = [planted("f16", "nn", m, n, 512, seed) for seed in range(4)]
+    rows, cols = sets[0][4], sets[0][5]
+    at = (rows[:, None], cols[None, :])
+    a, b = sets[0][0].clone(), sets[0][1].clone()
+    c, p, c2, p2 = (torch.empty((m, n), dtype=torch.float16, device="cuda") for _ in range(4))
+
+    def call(x, w, to, pre, stream):
+        pkg.linear(m, n, k, pkg.F16, x.data_ptr(), w.data_ptr(), pkg.F16, to.data_ptr(), pre=pre.data_ptr(), activation=pkg.ACT_RELU, stream=stream)
+    want = []
+    for s in sets:
+        call(s[0], s[1], c, p, 0)
+        pkg.device_status()
+        assert torch.equal(p[at] > 0, (s[2] @ s[3])[at] > 0)
+        want.append((c.clone(), p.clone()))
+    side, other, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call(a, b, c, p, torch.cuda.current_stream().cuda_stream)
+    for i, s in enumerate(sets):
+        a.copy_(s[0]), b.copy_(s[1])
+        torch.cuda.synchronize()
+        graph.replay()
+        call(sets[i - 1][0], sets[i - 1][1], c2, p2, other.cuda_stream)
+        torch.cuda.synchronize()
+        pkg.device_status()
+        assert torch.equal(c, want[i][0]) and torch.equal(p, want[i][1]) and torch.equal(c2, want[i - 1][0]) and torch.equal(p2, want[i - 1][1])
+
+
 def test_relu_border_beside_biases(cuda, pkg):
     """Sums that a bias of size one swallows are not the zeros of pruned blocks: elements next to zero in their rows and columns keep their side."""
     m, n = 296, 1032
