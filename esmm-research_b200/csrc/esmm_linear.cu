@@ -247,7 +247,7 @@ static_assert(LP_SMEM <= SMEM_LIMIT, "shared memory of a CTA");
 // The standard deviation is taken as (row's norm) (column's norm) / (norm) over a 32 x 64 piece, so that a column of small weights is not all border; a sum
 // that is exactly zero counts where it is the only one of its row and of its column in the piece (others are sums of zeros, as of pruned blocks).
 // An epilogue warp notes such elements of its pieces, as they lie rounded in its staging box, and the CTA sums them when its tiles are through, all epilogue
-// warps with a part of K each.  us with the values kept, silu / relu: 520 x 776 x 1032 fp16 9.2 / 11.1 (13.8 where an element is found), 2048 x 4096 x 11008 131 / 211
+// warps with a part of K each.  us with the values kept, silu / relu: 520 x 776 x 1032 fp16 8.7 / 9.9 (13 where an element is found), 2048 x 4096 x 11008 131 / 209
 // (some 800 elements, a column of B being 4096 lines of memory); summed by the warp alone within the piece 418, by a kernel of its own 220, and 17.5 for the small one.
 constexpr float LB_SHARE = 6e-9f, LB_SHARE_F8 = 3e-10f;
 constexpr float LB_WIDEST = 1e-3f;            // (from K = 167 thousand on, where 64-bit sums of all that may be off would take longer than the product)
@@ -268,7 +268,7 @@ __device__ __noinline__ double linear_sum64(const LinearParams &p, int row, int 
 {
     typedef typename LinearOperand<F8, BF16>::type operand_t;
     constexpr int U = 16;
-    double sum = 0.0;
+    double sum = 0.0, other = 0.0;
     if (bounds_ok(row < p.M && col < p.N, p.status, 66)) {   // checked build: site 66
         const operand_t *a = static_cast<const operand_t *>(p.A) + (size_t)row * p.a_row, *b = static_cast<const operand_t *>(p.B) + (size_t)col * p.b_col;
         for (long k0 = first; k0 < p.K; k0 += (long)step * U) {
@@ -280,9 +280,13 @@ __device__ __noinline__ double linear_sum64(const LinearParams &p, int row, int 
                 y[u] = b[k * p.b_k];
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) sum = fma(k0 + (long)step * u < p.K ? (double)linear_to_float(x[u]) : 0.0, (double)linear_to_float(y[u]), sum);
+            for (int u = 0; u < U; u += 2) {
+                sum = fma(k0 + (long)step * u < p.K ? (double)linear_to_float(x[u]) : 0.0, (double)linear_to_float(y[u]), sum);
+                other = fma(k0 + (long)step * (u + 1) < p.K ? (double)linear_to_float(x[u + 1]) : 0.0, (double)linear_to_float(y[u + 1]), other);
+            }
         }
     }
+    sum += other;
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     return sum;
@@ -313,11 +317,19 @@ __device__ __noinline__ int linear_note_border(const LinearParams &p, const char
     const int there = min(64, p.N - col0);
     auto value = [&](int j) { return to_float<out_t>(*reinterpret_cast<const out_t *>(mine + (((j >> 3) ^ (lane & 7)) << 4) + 2 * (j & 7))); };
     unsigned long long hit = 0, zero = 0;
-#pragma unroll 4
-    for (int j = 0; j < there; ++j) {
-        const float z = value(j);
-        hit |= (unsigned long long)(fabsf(z) < reach) << j;
-        zero |= (unsigned long long)(fabsf(z) < reach && z == cb[j]) << j;   // (only there: beside a bias of size one many a sum is lost in the rounding)
+#pragma unroll 1
+    for (int x = 0; x < there; x += 8) {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(mine + (((x >> 3) ^ (lane & 7)) << 4));
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+        unsigned below = 0, none = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 z = BF16 ? unpack_bf16(words[j]) : unpack_f16(words[j]), b = *reinterpret_cast<const float2 *>(cb + x + 2 * j);
+            below |= (unsigned)(fabsf(z.x) < reach) << (2 * j) | (unsigned)(fabsf(z.y) < reach) << (2 * j + 1);
+            none |= (unsigned)(z.x == b.x) << (2 * j) | (unsigned)(z.y == b.y) << (2 * j + 1);
+        }
+        hit |= (unsigned long long)below << x;
+        zero |= (unsigned long long)(below & none) << x;   // (only there: beside a bias of size one many a sum is lost in the rounding)
     }
     if (zero & (zero - 1)) hit &= ~zero;                         // not the only one of its row
     float whole = reach * reach;
